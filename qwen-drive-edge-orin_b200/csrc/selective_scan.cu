@@ -1,0 +1,63 @@
+// Selective scan over prompts: entry points, argument checks and the choice of kernel.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "gdn_ssm.h"
+#include "selective_scan.cuh"
+#include "ssm_common.cuh"
+
+namespace gdn {
+namespace ssm {
+
+constexpr size_t SCAN_WS_HEADER = 256;
+
+static bool scan_args_ok(const ScanArgs& a, int64_t rows) {
+    if (a.N < 0 || a.T < 0 || a.H < 1 || a.G < 1 || a.H % a.G != 0 || a.H > 65535 || a.N > 65535) return false;
+    if (a.P < 8 || a.P > 128 || a.P % 8 != 0 || a.NS < 8 || a.NS > 128 || a.NS % 8 != 0) return false;
+    if (a.xs < (int64_t)a.H * a.P || a.bs < (int64_t)a.G * a.NS || a.cs < (int64_t)a.G * a.NS || a.dts < a.H) return false;
+    if (a.xs % 8 != 0 || a.bs % 8 != 0 || a.cs % 8 != 0) return false;
+    if (a.N == 0) return true;
+    if (!a.A || !a.sf || !aligned_to(a.sf, 16) || !aligned_to(a.s0, 16)) return false;
+    if (rows > 0 && (!a.x || !a.dt || !a.B || !a.C || !a.y)) return false;
+    return aligned_to(a.x, 16) && aligned_to(a.B, 16) && aligned_to(a.C, 16) && aligned_to(a.y, 16);
+}
+
+}  // namespace ssm
+}  // namespace gdn
+
+extern "C" size_t selective_scan_workspace_size(int N, int T, int packed, int H, int P, int G, int n_state) {
+    return gdn::ssm::SCAN_WS_HEADER;
+}
+
+extern "C" cudaError_t selective_scan_prefill(const void* x, int64_t x_stride, const void* dt, int64_t dt_stride,
+                                              int dt_bf16, const float* A, const void* B, int64_t B_stride,
+                                              const void* C, int64_t C_stride, const float* D, const float* dt_bias,
+                                              int dt_softplus, const float* s0, void* y, float* sf,
+                                              const int* cu_seqlens, int N, int T, int H, int P, int G, int n_state,
+                                              void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+    using bf16 = __nv_bfloat16;
+    gdn::ssm::ScanArgs a{static_cast<const bf16*>(x), static_cast<const bf16*>(B), static_cast<const bf16*>(C), dt, A, D,
+                         dt_bias, s0, sf, static_cast<bf16*>(y), cu_seqlens, x_stride, dt_stride, B_stride, C_stride, N, T,
+                         H, P, G, n_state, dt_bf16, dt_softplus};
+    const int64_t rows = cu_seqlens ? T : (int64_t)N * T;
+    if (!gdn::ssm::scan_args_ok(a, rows)) return cudaErrorInvalidValue;
+    if (!workspace || workspace_bytes < selective_scan_workspace_size(N, T, cu_seqlens != nullptr, H, P, G, n_state))
+        return cudaErrorInvalidValue;
+    if (N == 0) return cudaSuccess;
+    return gdn::ssm::launch_scan_step(a, stream);
+}
+
+extern "C" cudaError_t selective_scan_decode(const void* x, int64_t x_stride, const void* dt, int64_t dt_stride,
+                                             int dt_bf16, const float* A, const void* B, int64_t B_stride, const void* C,
+                                             int64_t C_stride, const float* D, const float* dt_bias, int dt_softplus,
+                                             float* state, void* y, int N, int T, int H, int P, int G, int n_state,
+                                             cudaStream_t stream) {
+    using bf16 = __nv_bfloat16;
+    gdn::ssm::ScanArgs a{static_cast<const bf16*>(x), static_cast<const bf16*>(B), static_cast<const bf16*>(C), dt, A, D,
+                         dt_bias, state, state, static_cast<bf16*>(y), nullptr, x_stride, dt_stride, B_stride, C_stride, N,
+                         T, H, P, G, n_state, dt_bf16, dt_softplus};
+    if (!gdn::ssm::scan_args_ok(a, (int64_t)N * T)) return cudaErrorInvalidValue;
+    if (N == 0 || T == 0) return cudaSuccess;
+    return gdn::ssm::launch_scan_step(a, stream);
+}

@@ -13,6 +13,12 @@ and ``kernels/harness/chunk_delta.py``):
 * :func:`gated_rmsnorm` ``(o, z, w, eps=1e-6) -> y``
 * :func:`chunk_gated_delta_rule_fast` (transformers-compatible signature)
 
+State-space operators of hybrid layers (no counterparts in the reference):
+
+* :func:`causal_conv_prefill`, :func:`causal_conv_prefill_varlen`, :func:`causal_conv_decode`
+* :func:`selective_scan_prefill`, :func:`selective_scan_prefill_varlen`, :func:`selective_scan_decode`
+* :func:`gated_group_rmsnorm` ``(x, z, w, groups=1, eps=1e-6) -> y``
+
 Every call goes through the C-ABI shared library ``libgdn_b200.so`` built
 from ``csrc/``; there is no CPU or library fallback.
 """
@@ -32,5 +38,14 @@ from .binding import (  # noqa: F401
     chunk_gated_delta_rule_fast,
     workspace_size,
     GdnError,
+)
+from .ssm import (  # noqa: F401
+    causal_conv_prefill,
+    causal_conv_prefill_varlen,
+    causal_conv_decode,
+    selective_scan_prefill,
+    selective_scan_prefill_varlen,
+    selective_scan_decode,
+    gated_group_rmsnorm,
 )
 from ._lib import load_library, library_path  # noqa: F401

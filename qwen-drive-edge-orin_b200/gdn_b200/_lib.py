@@ -17,7 +17,7 @@ _lib = None
 c_void_p, c_int, c_float, c_size_t, c_int64 = (ctypes.c_void_p, ctypes.c_int, ctypes.c_float,
                                                ctypes.c_size_t, ctypes.c_int64)
 
-# name -> (restype, argtypes); mirrors include/gdn_prefill.h
+# name -> (restype, argtypes); mirrors include/gdn_prefill.h and include/gdn_ssm.h
 SIGNATURES = {
     "deltanet_prefill_workspace_size": (c_size_t, [c_int] * 6),
     "deltanet_prefill_debug_workspace_size": (c_size_t, [c_int] * 6),
@@ -40,6 +40,18 @@ SIGNATURES = {
     "gdn_run_chunk_prefill": (c_int, [c_void_p, c_void_p]),
     "deltanet_recurrent_decode": (c_int, [c_void_p] * 7 + [c_float, c_void_p, c_void_p] + [c_int] * 6 + [c_void_p]),
     "gated_rmsnorm_forward": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_float, c_int, c_void_p]),
+    # include/gdn_ssm.h
+    "causal_conv_prefill": (c_int, [c_void_p, c_int64] + [c_void_p] * 6 + [c_int] * 6 + [c_void_p]),
+    "causal_conv_decode": (c_int, [c_void_p, c_int64] + [c_void_p] * 4 + [c_int] * 6 + [c_void_p]),
+    "selective_scan_workspace_size": (c_size_t, [c_int] * 7),
+    "selective_scan_prefill": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64,
+                                       c_void_p, c_int64, c_void_p, c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 6
+                               + [c_void_p, c_size_t, c_void_p]),
+    "selective_scan_decode": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64,
+                                      c_void_p, c_int64, c_void_p, c_void_p, c_int] + [c_void_p] * 2 + [c_int] * 6
+                              + [c_void_p]),
+    "gated_group_rmsnorm_forward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int,
+                                            c_int, c_float, c_int, c_void_p]),
     "deltanet_read_status": (c_int, [c_void_p, ctypes.POINTER(c_int), c_int, c_void_p]),
     "deltanet_noalloc_read_status": (c_int, [ctypes.POINTER(c_int), c_int, c_void_p]),
     "gdn_b200_version": (ctypes.c_char_p, []),

@@ -1,0 +1,275 @@
+"""Torch-facing binding of the state-space operators (include/gdn_ssm.h): the short causal
+convolution, the selective scan and the gated group norm of hybrid layers, for prompts (batched
+or packed) and for single tokens. No counterparts in the reference; same conventions as the gated
+delta rule's entries (``binding.py``): ValueError for bad arguments, GdnError for a launch that
+failed, torch's current CUDA stream of the inputs' device, outputs allocated with torch, no autograd.
+
+Inputs may be slices of a wider projection (a row stride above the row's width); other layouts
+are copied to contiguous memory first.
+"""
+from __future__ import annotations
+
+import torch
+
+from ._lib import load_library
+from .binding import _check, _same_device, _workspace
+
+__all__ = ["causal_conv_prefill", "causal_conv_prefill_varlen", "causal_conv_decode", "selective_scan_prefill",
+           "selective_scan_prefill_varlen", "selective_scan_decode", "gated_group_rmsnorm"]
+
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _call(dev, what, fn, *args):
+    """fn(*args, stream) on torch's current stream of ``dev``."""
+    if dev.index == torch.cuda.current_device():
+        code = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            code = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if code:
+        _check(code, what)
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rows(t, lead, align=1):
+    """(t, row stride in elements): t with its ``lead`` leading dims as evenly spaced rows and its
+    other dims contiguous inside a row, t itself where that holds and pointer and stride are
+    multiples of ``align`` elements, else a contiguous copy."""
+    width = 1
+    for d in range(t.dim() - 1, lead - 1, -1):
+        if t.shape[d] != 1 and t.stride(d) != width:
+            return _packed_rows(t, lead, align)
+        width *= t.shape[d]
+    stride, rows = None, 1
+    for d in range(lead - 1, -1, -1):
+        if t.shape[d] == 1:
+            continue
+        if stride is None:
+            stride = t.stride(d)
+        elif t.stride(d) != stride * rows:
+            return _packed_rows(t, lead, align)
+        rows *= t.shape[d]
+    if stride is None:  # one row
+        stride = width
+    if stride < width or stride % align or t.data_ptr() % (align * t.element_size()):
+        return _packed_rows(t, lead, align)
+    return t, stride
+
+
+def _packed_rows(t, lead, align):
+    t = t.contiguous()
+    if t.data_ptr() % (align * t.element_size()):
+        t = t.clone()
+    width = 1
+    for n in t.shape[lead:]:
+        width *= n
+    return t, width
+
+
+def _vector(t, n, dtype, name, dev):
+    if t is None:
+        return None
+    if t.dtype != dtype or tuple(t.shape) != (n,):
+        raise ValueError(f"{name} must be {dtype} of shape [{n}]")
+    if t.device != dev:
+        raise ValueError("all tensors must be on the same CUDA device")
+    return t.contiguous()
+
+
+def _initial(s0, shape, dtype, dev):
+    """The initial state as a contiguous, 16-byte aligned tensor of ``dtype`` (or None)."""
+    if s0 is None:
+        return None
+    if tuple(s0.shape) != tuple(shape):
+        raise ValueError(f"initial state must have shape {tuple(shape)}, got {tuple(s0.shape)}")
+    s0 = s0.to(device=dev, dtype=dtype).contiguous()
+    return s0 if s0.data_ptr() % 16 == 0 else s0.clone()
+
+
+def _offsets(cu_seqlens, dev):
+    if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or not cu_seqlens.is_cuda or cu_seqlens.numel() < 1:
+        raise ValueError("cu_seqlens must be a 1-D int32 CUDA tensor of at least one element")
+    if cu_seqlens.device != dev:
+        raise ValueError("all tensors must be on the same CUDA device")
+    return cu_seqlens.contiguous()
+
+
+# ---------------------------------------------------------------- causal convolution
+def _check_conv(x, w, bias, packed=False):
+    if not x.is_cuda or not w.is_cuda:
+        raise ValueError("all inputs must be CUDA tensors")
+    if x.dtype not in _DTYPES or w.dtype != x.dtype:
+        raise ValueError("x and w must share dtype fp16, bf16 or fp32")
+    if x.dim() != 3 or w.dim() != 2 or w.shape[0] != x.shape[2]:
+        raise ValueError("bad shapes: x must be [B, T, C] and w [C, W]")
+    if not 2 <= w.shape[1] <= 4:
+        raise ValueError("only 2 to 4 taps are supported")
+    if x.shape[2] < 1:
+        raise ValueError("x needs at least one channel")
+    if packed and x.shape[0] != 1:
+        raise ValueError("varlen inputs are packed: B must be 1")
+    dev = _same_device(x, w)
+    return dev, _vector(bias, x.shape[2], x.dtype, "bias", dev)
+
+
+def _conv_prefill(x, w, bias, s0, silu, cu):
+    dev, bias = _check_conv(x, w, bias, cu is not None)
+    B, T, C = x.shape
+    W = w.shape[1]
+    if cu is not None:
+        cu = _offsets(cu, dev)
+    n = B if cu is None else cu.numel() - 1
+    s0 = _initial(s0, (n, W - 1, C), x.dtype, dev)
+    x, stride = _rows(x, 2)
+    w = w.contiguous()
+    y = torch.empty((B, T, C), dtype=x.dtype, device=dev)
+    sf = torch.empty((n, W - 1, C), dtype=x.dtype, device=dev)
+    _call(dev, "causal_conv_prefill", load_library().causal_conv_prefill, _p(x), stride, _p(w), _p(bias), _p(s0), _p(y),
+          _p(sf), _p(cu), n, T, C, W, int(bool(silu)), _DTYPES[x.dtype])
+    return [y, sf]
+
+
+def causal_conv_prefill(x, w, bias=None, s0=None, silu: bool = True):
+    """Short causal depthwise convolution over prompts: [y [B,T,C], final state [B,W-1,C]].
+
+    y[t, c] = act(bias[c] + sum_j w[c, j] x[t - W + 1 + j, c]), act = silu unless ``silu`` is false.
+    x [B,T,C], w [C,W] with 2 to 4 taps, bias [C], all fp16, bf16 or fp32 (fp32 math). Inputs before
+    the start are ``s0`` [B,W-1,C] (oldest first) or zeros; the final state is the last W-1 inputs.
+    """
+    return _conv_prefill(x, w, bias, s0, silu, None)
+
+
+def causal_conv_prefill_varlen(x, w, cu_seqlens, bias=None, s0=None, silu: bool = True):
+    """``causal_conv_prefill`` of packed sequences (B = 1): [y [1,T,C], final states [N,W-1,C]].
+
+    Sequence i covers tokens [cu[i], cu[i+1]) of int32 ``cu_seqlens`` [N+1] (on the device) and starts
+    from s0[i] or zeros. Tokens that no sequence covers are not computed: their rows of y hold no
+    defined values.
+    """
+    return _conv_prefill(x, w, bias, s0, silu, cu_seqlens)
+
+
+def causal_conv_decode(x, w, state, bias=None, silu: bool = True):
+    """The convolution of the next token(s) x [B,T,C] (T usually 1): returns y [B,T,C]; ``state``
+    [B,W-1,C] (a prefill's final state, x's dtype, contiguous) is updated in place."""
+    dev, bias = _check_conv(x, w, bias)
+    B, T, C = x.shape
+    W = w.shape[1]
+    if state.dtype != x.dtype or not state.is_contiguous() or tuple(state.shape) != (B, W - 1, C):
+        raise ValueError(f"state must be a contiguous tensor of x's dtype and shape {(B, W - 1, C)}")
+    _same_device(x, state)
+    x, stride = _rows(x, 2)
+    w = w.contiguous()
+    y = torch.empty((B, T, C), dtype=x.dtype, device=dev)
+    _call(dev, "causal_conv_decode", load_library().causal_conv_decode, _p(x), stride, _p(w), _p(bias), _p(state), _p(y),
+          B, T, C, W, int(bool(silu)), _DTYPES[x.dtype])
+    return y
+
+
+# ---------------------------------------------------------------- selective scan
+def _check_scan(x, dt, A, B, C, D, dt_bias, packed=False):
+    if not (x.is_cuda and dt.is_cuda and A.is_cuda and B.is_cuda and C.is_cuda):
+        raise ValueError("all inputs must be CUDA tensors")
+    dev = _same_device(x, dt, A, B, C)
+    if not (x.dtype == B.dtype == C.dtype == torch.bfloat16):
+        raise ValueError("x/B/C must be bf16")
+    if dt.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("dt must be fp32 or bf16")
+    if x.dim() != 4 or B.dim() != 4 or C.dim() != 4 or dt.dim() != 3:
+        raise ValueError("bad ranks: x must be 4-D [B,T,H,P], B/C 4-D [B,T,G,N], dt 3-D [B,T,H]")
+    b, T, H, P = x.shape
+    G, N = B.shape[2], B.shape[3]
+    if B.shape[:2] != (b, T) or C.shape != B.shape or dt.shape != (b, T, H):
+        raise ValueError("shape mismatch between x/dt/B/C")
+    if G < 1 or H < 1 or H % G != 0:
+        raise ValueError("H must be a multiple of G")
+    if not (8 <= P <= 128 and P % 8 == 0 and 8 <= N <= 128 and N % 8 == 0):
+        raise ValueError("P and N must be multiples of 8 up to 128")
+    if packed and b != 1:
+        raise ValueError("varlen inputs are packed: B must be 1")
+    A = _vector(A, H, torch.float32, "A", dev)
+    D = _vector(D, H, torch.float32, "D", dev)
+    dt_bias = _vector(dt_bias, H, torch.float32, "dt_bias", dev)
+    return dev, (b, T, H, P, G, N), A, D, dt_bias
+
+
+def _scan_prefill(x, dt, A, B, C, D, dt_bias, s0, dt_softplus, cu):
+    dev, (b, T, H, P, G, N), A, D, dt_bias = _check_scan(x, dt, A, B, C, D, dt_bias, cu is not None)
+    if cu is not None:
+        cu = _offsets(cu, dev)
+    n = b if cu is None else cu.numel() - 1
+    s0 = _initial(s0, (n, H, P, N), torch.float32, dev)
+    (x, xs), (dt, dts), (B, bs), (C, cs) = _rows(x, 2, 8), _rows(dt, 2), _rows(B, 2, 8), _rows(C, 2, 8)
+    y = torch.empty((b, T, H, P), dtype=torch.bfloat16, device=dev)
+    sf = torch.empty((n, H, P, N), dtype=torch.float32, device=dev)
+    lib = load_library()
+    nbytes = lib.selective_scan_workspace_size(n, T, int(cu is not None), H, P, G, N)
+    ws = _workspace(dev, nbytes)
+    _call(dev, "selective_scan_prefill", lib.selective_scan_prefill, _p(x), xs, _p(dt), dts, int(dt.dtype == torch.bfloat16),
+          _p(A), _p(B), bs, _p(C), cs, _p(D), _p(dt_bias), int(bool(dt_softplus)), _p(s0), _p(y), _p(sf), _p(cu), n, T, H, P,
+          G, N, _p(ws), ws.numel())
+    return [y, sf]
+
+
+def selective_scan_prefill(x, dt, A, B, C, D=None, dt_bias=None, s0=None, dt_softplus: bool = False):
+    """Selective state space scan over prompts: [y (bf16 [B,T,H,P]), final state (fp32 [B,H,P,N])].
+
+    Per head h of group g = h // (H // G), with d = dt + dt_bias (softplus'ed if ``dt_softplus``):
+        S <- exp(d A) S + d x B^T;   y = S C + D x.
+    x bf16 [B,T,H,P], dt fp32 or bf16 [B,T,H], B/C bf16 [B,T,G,N], A, D, dt_bias fp32 [H], initial
+    state s0 fp32 [B,H,P,N] or zeros. P and N are multiples of 8 up to 128; d A <= 0 is expected.
+    """
+    return _scan_prefill(x, dt, A, B, C, D, dt_bias, s0, dt_softplus, None)
+
+
+def selective_scan_prefill_varlen(x, dt, A, B, C, cu_seqlens, D=None, dt_bias=None, s0=None, dt_softplus: bool = False):
+    """``selective_scan_prefill`` of packed sequences (B = 1): [y [1,T,H,P], final states [N,H,P,N]].
+
+    ``cu_seqlens`` as in ``chunk_prefill_varlen``; sequence i starts from s0[i] or zeros. Tokens that
+    no sequence covers are not computed: their rows of y hold no defined values.
+    """
+    return _scan_prefill(x, dt, A, B, C, D, dt_bias, s0, dt_softplus, cu_seqlens)
+
+
+def selective_scan_decode(x, dt, A, B, C, state, D=None, dt_bias=None, dt_softplus: bool = False):
+    """The scan of the next token(s) x [B,T,H,P] (T usually 1), shapes as in ``selective_scan_prefill``:
+    returns y; the fp32 ``state`` [B,H,P,N] (e.g. a prefill's final state) is updated in place."""
+    dev, (b, T, H, P, G, N), A, D, dt_bias = _check_scan(x, dt, A, B, C, D, dt_bias)
+    if state.dtype != torch.float32 or not state.is_contiguous() or tuple(state.shape) != (b, H, P, N):
+        raise ValueError("state must be a contiguous fp32 [B, H, P, N] tensor")
+    _same_device(x, state)
+    if state.data_ptr() % 16:
+        raise ValueError("state must be 16-byte aligned")
+    (x, xs), (dt, dts), (B, bs), (C, cs) = _rows(x, 2, 8), _rows(dt, 2), _rows(B, 2, 8), _rows(C, 2, 8)
+    y = torch.empty((b, T, H, P), dtype=torch.bfloat16, device=dev)
+    _call(dev, "selective_scan_decode", load_library().selective_scan_decode, _p(x), xs, _p(dt), dts,
+          int(dt.dtype == torch.bfloat16), _p(A), _p(B), bs, _p(C), cs, _p(D), _p(dt_bias), int(bool(dt_softplus)), _p(state),
+          _p(y), b, T, H, P, G, N)
+    return y
+
+
+# ---------------------------------------------------------------- gated group norm
+def gated_group_rmsnorm(x, z, w, groups: int = 1, eps: float = 1e-6):
+    """Gated RMSNorm over channel groups with the gate before the norm, over the last dim:
+    u = x silu(z); y = w u rsqrt(mean_group(u^2) + eps). x, z [..., C], w [C], all fp16, bf16 or fp32;
+    ``groups`` divides C. (``gated_rmsnorm`` has the gate behind the norm.)"""
+    if x.dtype not in _DTYPES or z.dtype != x.dtype or w.dtype != x.dtype:
+        raise ValueError("x, z, w must share dtype fp16, bf16 or fp32")
+    if not (x.is_cuda and z.is_cuda and w.is_cuda):
+        raise ValueError("all inputs must be CUDA tensors")
+    if x.dim() < 1 or z.shape != x.shape or w.dim() != 1 or w.shape[0] != x.shape[-1]:
+        raise ValueError("z must match x and w must be [C]")
+    C = x.shape[-1]
+    if groups < 1 or C < 1 or C % groups != 0:
+        raise ValueError("groups must divide the last dim")
+    dev = _same_device(x, z, w)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    (x, xs), (z, zs) = _rows(x, x.dim() - 1), _rows(z, z.dim() - 1)
+    w = w.contiguous()
+    _call(dev, "gated_group_rmsnorm_forward", load_library().gated_group_rmsnorm_forward, _p(x), xs, _p(z), zs, _p(w), _p(y),
+          x.numel() // C, C, int(groups), float(eps), _DTYPES[x.dtype])
+    return y

@@ -1,0 +1,119 @@
+"""Host-side checks of the state-space operators: the library exports every symbol that
+include/gdn_ssm.h declares, and bad arguments are refused before any device work."""
+from __future__ import annotations
+
+import ctypes
+import re
+
+import pytest
+import torch
+
+from conftest import ROOT
+import gdn_b200
+from gdn_b200 import _lib
+from gdn_b200.ssm import _rows
+
+INVALID = 1  # cudaErrorInvalidValue
+P = ctypes.c_void_p(1 << 20)
+
+
+def test_library_exports_every_declared_symbol():
+    text = re.sub(r"/\*.*?\*/", "", (ROOT / "include" / "gdn_ssm.h").read_text(), flags=re.S)
+    names = set(re.findall(r"\b([a-z_][a-z0-9_]*)\s*\(", text)) - {"defined"}
+    assert {"causal_conv_prefill", "selective_scan_prefill", "gated_group_rmsnorm_forward"} <= names
+    raw = ctypes.CDLL(str(_lib.library_path()))
+    for n in names:
+        assert hasattr(raw, n) and n in _lib.SIGNATURES, n
+
+
+def _conv(**kw):
+    a = dict(x=P, xs=64, w=P, bias=None, s0=None, y=P, sf=P, cu=None, N=1, T=4, C=64, W=4, silu=1, dtype=1)
+    a.update(kw)
+    return gdn_b200.load_library().causal_conv_prefill(*a.values(), None)
+
+
+@pytest.mark.parametrize("bad", [dict(x=None), dict(w=None), dict(y=None), dict(sf=None), dict(xs=63), dict(N=-1),
+                                 dict(T=-1), dict(C=0), dict(W=1), dict(W=5), dict(dtype=3), dict(dtype=-1)])
+def test_conv_refuses(bad):
+    assert _conv(**bad) == INVALID
+
+
+def test_empty_calls_are_no_ops():
+    lib = gdn_b200.load_library()
+    assert _conv(N=0) == 0
+    assert lib.causal_conv_decode(P, 64, P, None, P, P, 2, 0, 64, 4, 1, 1, None) == 0
+    assert lib.gated_group_rmsnorm_forward(P, 64, P, 64, P, P, 0, 64, 1, 1e-6, 1, None) == 0
+    assert _scan(N=0) == 0
+    assert _scan_decode(N=0) == 0 and _scan_decode(T=0) == 0
+
+
+def _scan(**kw):
+    a = dict(x=P, xs=128, dt=P, dts=2, dtb=0, A=P, B=P, bs=128, C=P, cs=128, D=None, bias=None, sp=1, s0=None, y=P, sf=P,
+             cu=None, N=1, T=4, H=2, P=64, G=1, NS=128, ws=P, wsb=1 << 30)
+    a.update(kw)
+    return gdn_b200.load_library().selective_scan_prefill(*a.values(), None)
+
+
+def _scan_decode(**kw):
+    a = dict(x=P, xs=128, dt=P, dts=2, dtb=0, A=P, B=P, bs=128, C=P, cs=128, D=None, bias=None, sp=1, state=P, y=P,
+             N=1, T=4, H=2, P=64, G=1, NS=128)
+    a.update(kw)
+    return gdn_b200.load_library().selective_scan_decode(*a.values(), None)
+
+
+COMMON = [dict(x=None), dict(dt=None), dict(A=None), dict(B=None), dict(C=None), dict(y=None), dict(xs=127), dict(xs=132),
+          dict(bs=124), dict(cs=130), dict(dts=1), dict(N=-1), dict(T=-1), dict(H=0), dict(G=0), dict(H=3, G=2), dict(P=0),
+          dict(P=60), dict(P=136), dict(NS=4), dict(NS=100), dict(NS=136), dict(N=65536), dict(H=65536, P=8, xs=1 << 20),
+          dict(x=ctypes.c_void_p((1 << 20) + 8)), dict(B=ctypes.c_void_p((1 << 20) + 2))]
+
+
+@pytest.mark.parametrize("bad", COMMON + [dict(sf=None), dict(ws=None), dict(wsb=128), dict(s0=ctypes.c_void_p((1 << 20) + 4))])
+def test_scan_refuses(bad):
+    assert _scan(**bad) == INVALID
+
+
+@pytest.mark.parametrize("bad", COMMON + [dict(state=None), dict(state=ctypes.c_void_p((1 << 20) + 4))])
+def test_scan_decode_refuses(bad):
+    assert _scan_decode(**bad) == INVALID
+
+
+@pytest.mark.parametrize("bad", [dict(x=None), dict(z=None), dict(w=None), dict(y=None), dict(rows=-1), dict(C=0),
+                                 dict(groups=0), dict(groups=3), dict(dtype=3), dict(xs=63), dict(zs=63)])
+def test_group_norm_refuses(bad):
+    a = dict(x=P, xs=64, z=P, zs=64, w=P, y=P, rows=4, C=64, groups=2, eps=1e-6, dtype=1)
+    a.update(bad)
+    assert gdn_b200.load_library().gated_group_rmsnorm_forward(*a.values(), None) == INVALID
+
+
+def test_binding_refuses_cpu_tensors():
+    bf = torch.bfloat16
+    x, w = torch.zeros(1, 4, 8, dtype=bf), torch.zeros(8, 4, dtype=bf)
+    with pytest.raises(ValueError):
+        gdn_b200.causal_conv_prefill(x, w)
+    with pytest.raises(ValueError):
+        gdn_b200.causal_conv_decode(x, w, torch.zeros(1, 3, 8, dtype=bf))
+    with pytest.raises(ValueError):
+        gdn_b200.gated_group_rmsnorm(x, x, torch.zeros(8, dtype=bf))
+    xs, b, dt, a = torch.zeros(1, 4, 2, 64, dtype=bf), torch.zeros(1, 4, 1, 64, dtype=bf), torch.zeros(1, 4, 2), torch.zeros(2)
+    with pytest.raises(ValueError):
+        gdn_b200.selective_scan_prefill(xs, dt, a, b, b)
+    with pytest.raises(ValueError):
+        gdn_b200.selective_scan_decode(xs, dt, a, b, b, torch.zeros(1, 2, 64, 64))
+
+
+def test_rows_keeps_slices_and_copies_the_rest():
+    wide = torch.arange(2 * 3 * 20.).reshape(2, 3, 20)
+    t, s = _rows(wide[..., 4:12], 2)
+    assert t.data_ptr() == wide[..., 4:12].data_ptr() and s == 20
+    t, s = _rows(wide.transpose(0, 1), 2)  # tokens not evenly spaced
+    assert s == 20 and torch.equal(t, wide.transpose(0, 1)) and t.is_contiguous()
+    t, s = _rows(wide[..., ::2], 2)  # channels not contiguous
+    assert s == 10 and torch.equal(t, wide[..., ::2])
+    t, s = _rows(wide[:1, :1].expand(2, 3, 20), 2)  # a broadcast input
+    assert s == 20 and t.is_contiguous()
+    t, s = _rows(wide[:, 1:2, :8], 2)  # one token per sequence
+    assert s == 60 and t.data_ptr() == wide[0, 1].data_ptr()
+    t, s = _rows(wide.reshape(-1)[1:113].reshape(14, 8), 1, 4)  # contiguous, misaligned
+    assert s == 8 and t.data_ptr() % 16 == 0
+    t, s = _rows(torch.zeros(2, 0, 8), 2)
+    assert s >= 8
