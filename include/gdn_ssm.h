@@ -51,16 +51,18 @@ cudaError_t causal_conv_decode(const void* x, int64_t x_stride, const void* w, c
  * uses group h / (H / G); dt [rows, H] fp32 (dt_bf16 = 0) or bf16 (1); A, D (or NULL), dt_bias (or
  * NULL) fp32 [H]; y bf16 [rows, H, P]; s0 (or NULL: zeros) and sf fp32 [N, H, P, N_STATE].
  * d A <= 0 is expected (a decay). P and N_STATE are multiples of 8 up to 128; x, B, C rows
- * 16-byte aligned. sf may be s0 itself; otherwise they must not overlap.
- * workspace: selective_scan_workspace_size(...) bytes for the same sizes on the same device; its
- * first 256 bytes hold the status word (deltanet_read_status) and must be zero before first use;
- * calls that may overlap in time need workspaces of their own. */
-size_t selective_scan_workspace_size(int N, int T, int packed, int H, int P, int G, int n_state);
+ * 16-byte aligned. sf must not overlap s0.
+ * workspace: at least 256 bytes, zero before its first use, whose first word is the status word
+ * (deltanet_read_status); calls may share it. scratch: selective_scan_scratch_size(...) bytes for the
+ * same sizes on the same device, 256-byte aligned (NULL where that is 0); calls that may overlap in
+ * time need scratch of their own. */
+size_t selective_scan_scratch_size(int N, int T, int packed, int H, int P, int G, int n_state);
 cudaError_t selective_scan_prefill(const void* x, int64_t x_stride, const void* dt, int64_t dt_stride, int dt_bf16,
                                    const float* A, const void* B, int64_t B_stride, const void* C, int64_t C_stride,
                                    const float* D, const float* dt_bias, int dt_softplus, const float* s0, void* y,
                                    float* sf, const int* cu_seqlens, int N, int T, int H, int P, int G, int n_state,
-                                   void* workspace, size_t workspace_bytes, cudaStream_t stream);
+                                   void* workspace, size_t workspace_bytes, void* scratch, size_t scratch_bytes,
+                                   cudaStream_t stream);
 
 /* The next T tokens (usually one) of `N` sequences, x [N, T, H, P], with the state [N, H, P, N_STATE]
  * read and updated in place. Continues a prefill from its final state. */

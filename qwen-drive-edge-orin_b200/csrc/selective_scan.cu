@@ -10,7 +10,16 @@
 namespace gdn {
 namespace ssm {
 
-constexpr size_t SCAN_WS_HEADER = 256;
+// Up to this many tokens a prompt runs token by token.
+constexpr int STEP_TOKENS = 6;
+
+static int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return 148;
+    return sms;
+}
 
 static bool scan_args_ok(const ScanArgs& a, int64_t rows) {
     if (a.N < 0 || a.T < 0 || a.H < 1 || a.G < 1 || a.H % a.G != 0 || a.H > 65535 || a.N > 65535) return false;
@@ -26,8 +35,11 @@ static bool scan_args_ok(const ScanArgs& a, int64_t rows) {
 }  // namespace ssm
 }  // namespace gdn
 
-extern "C" size_t selective_scan_workspace_size(int N, int T, int packed, int H, int P, int G, int n_state) {
-    return gdn::ssm::SCAN_WS_HEADER;
+extern "C" size_t selective_scan_scratch_size(int N, int T, int packed, int H, int P, int G, int n_state) {
+    using namespace gdn::ssm;
+    if (N <= 0 || T <= STEP_TOKENS || H < 1 || G < 1 || H % G != 0 || P < 1) return 0;
+    const ChunkPlan pl = plan_scan_chunks(N, T, packed != 0, H, P, G, sm_count());
+    return pl.log_bytes + pl.part_bytes;
 }
 
 extern "C" cudaError_t selective_scan_prefill(const void* x, int64_t x_stride, const void* dt, int64_t dt_stride,
@@ -35,17 +47,23 @@ extern "C" cudaError_t selective_scan_prefill(const void* x, int64_t x_stride, c
                                               const void* C, int64_t C_stride, const float* D, const float* dt_bias,
                                               int dt_softplus, const float* s0, void* y, float* sf,
                                               const int* cu_seqlens, int N, int T, int H, int P, int G, int n_state,
-                                              void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+                                              void* workspace, size_t workspace_bytes, void* scratch,
+                                              size_t scratch_bytes, cudaStream_t stream) {
     using bf16 = __nv_bfloat16;
     gdn::ssm::ScanArgs a{static_cast<const bf16*>(x), static_cast<const bf16*>(B), static_cast<const bf16*>(C), dt, A, D,
                          dt_bias, s0, sf, static_cast<bf16*>(y), cu_seqlens, x_stride, dt_stride, B_stride, C_stride, N, T,
                          H, P, G, n_state, dt_bf16, dt_softplus};
     const int64_t rows = cu_seqlens ? T : (int64_t)N * T;
     if (!gdn::ssm::scan_args_ok(a, rows)) return cudaErrorInvalidValue;
-    if (!workspace || workspace_bytes < selective_scan_workspace_size(N, T, cu_seqlens != nullptr, H, P, G, n_state))
-        return cudaErrorInvalidValue;
+    if (!workspace || workspace_bytes < 256) return cudaErrorInvalidValue;
     if (N == 0) return cudaSuccess;
-    return gdn::ssm::launch_scan_step(a, stream);
+    if (T <= gdn::ssm::STEP_TOKENS) return gdn::ssm::launch_scan_step(a, stream);
+    if (rows > 0x7fffffffLL - 128) return cudaErrorInvalidValue;  // token rows are 32-bit tile coordinates
+    const gdn::ssm::ChunkPlan pl =
+        gdn::ssm::plan_scan_chunks(N, T, cu_seqlens != nullptr, H, P, G, gdn::ssm::sm_count());
+    if (pl.part_bytes > 0 && (!scratch || !gdn::aligned_to(scratch, 256) || scratch_bytes < pl.log_bytes + pl.part_bytes))
+        return cudaErrorInvalidValue;
+    return gdn::ssm::launch_scan_chunks(a, pl, rows, workspace, scratch, stream);
 }
 
 extern "C" cudaError_t selective_scan_decode(const void* x, int64_t x_stride, const void* dt, int64_t dt_stride,

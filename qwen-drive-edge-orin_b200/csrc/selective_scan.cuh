@@ -25,6 +25,18 @@ struct ScanArgs {
 // Token by token against a state in registers (one launch); any supported size.
 cudaError_t launch_scan_step(const ScanArgs& a, cudaStream_t stream);
 
+// In 128-token chunks on the tensor cores. The plan: units = slot pairs (two tiles of up to 64
+// channels) over all groups, segments over all sequences (seg_tokens = 0: one each), and the
+// scratch for the segments' states and log decays.
+struct ChunkPlan {
+    int pairs, units, seg_tokens;
+    int64_t segments;
+    size_t part_bytes, log_bytes;
+};
+ChunkPlan plan_scan_chunks(int N, int T, bool packed, int H, int P, int G, int sms);
+cudaError_t launch_scan_chunks(const ScanArgs& a, const ChunkPlan& pl, int64_t rows, void* workspace, void* scratch,
+                               cudaStream_t stream);
+
 // Step size of (row, head) before the bias and the softplus.
 __device__ __forceinline__ float scan_dt(const ScanArgs& a, int64_t row, int h) {
     return a.dt_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.dt)[row * a.dts + h])

@@ -1,0 +1,842 @@
+// Selective scan over prompts in 128-token chunks on the tensor cores (tcgen05, TMEM, TMA).
+//
+// With a_t = d_t A (log decay) and c_i the inclusive sum of a over a chunk, the recurrence
+// S <- e^{a_t} S + d_t x_t B_t^T, y_t = S C_t + D x_t is, over one chunk with entry state S,
+//   G      = C B^T                                              [128 x 128]  (shared by the heads of a group)
+//   y      = diag(e^{c}) (C S^T) + M X + D X,   M_ij = G_ij e^{c_i - c_j} d_j for j <= i, else 0
+//   S^T   <- e^{c_L} S^T + B^T X',              X'_j = e^{c_L - c_j} d_j x_j
+// all four products with 128 rows.
+//
+// A CTA owns one segment of a sequence and two "slots" of a group: a slot is one head's tile of up to
+// 64 channels (a head of 128 is two slots). The two share the B and C tiles and G, and stand side by
+// side in the N = 128 columns of the inter-chunk and state products. Per chunk the tensor pipe runs
+// inter (C S^T), state (B^T X', three products, below), intra (M X) and the next chunk's G, in this
+// order, so that it has work while the warps form M, X' and the next state operand.
+//   warps 0-7   slot 0 / slot 1: M (bf16) from G into TMEM, the A operand of M X; Y <- e^c Y; output tile
+//   warps 8-15  slot 0 / slot 1: X' pieces of 16 tokens into a ring; the state S^T (fp32, TMEM-resident):
+//               its bf16 copy (operand of C S^T) and its decay
+//   warp 16     issues every MMA (one thread); warp 17 every TMA load; warp 18 the gates; warp 19 the
+//               TMA stores of the output tiles
+//
+// Precision. G and all sums are fp32. M and the state operand of C S^T are rounded to bf16 once (y is
+// a bf16 output: together 1.0 of its own rounding error). The state itself is an fp32 output and carries
+// over thousands of tokens: X' is split exactly into three bf16 terms (8 + 8 + 8 bits of an fp32 value),
+// so its products are those of fp32 operands.
+//
+// Decays are kept as base-2 logarithms, relative to 32-token blocks: e^{c_i - c_j} across blocks is
+// a row factor times a column factor, both at most 1 (one exponential per row and block), and inside
+// the diagonal block an exponential per element.
+//
+// Bound: 32 KB of x and y per slot pair and chunk (5.1 us / 148 at the copy bandwidth) against
+// 3072 tensor cycles.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <string.h>
+
+#include <atomic>
+#include <mutex>
+
+#include "gdn_common.cuh"
+#include "gdn_ssm.h"
+#include "selective_scan.cuh"
+#include "ssm_common.cuh"
+
+namespace gdn {
+namespace ssm {
+
+constexpr int CH = 128;      // tokens per chunk
+constexpr int TILE = 64;     // channels per slot
+constexpr int PIECE = 16;    // tokens per piece of X'
+constexpr int PIECES = CH / PIECE;
+constexpr int WARPS = 20;
+constexpr int CHUNK_THREADS = 32 * WARPS;
+
+// ---- shared memory (bytes from a 1024-aligned base); bf16 tiles in the 128-byte swizzle TMA writes:
+// panels of 64 columns, rows of 128 bytes
+constexpr uint32_t PANEL = CH * 128;                 // 16 KB
+constexpr uint32_t OFF_B = 0;                        // 2 buffers x 2 panels [128 tokens][64 state]
+constexpr uint32_t OFF_C = OFF_B + 4 * PANEL;        // 2 panels
+constexpr uint32_t OFF_X = OFF_C + 2 * PANEL;        // 2 buffers x 2 slots [128 tokens][64 channels]; becomes y
+constexpr uint32_t OFF_S = OFF_X + 4 * PANEL;        // 2 slots [128 state][64 channels]
+constexpr uint32_t SUB = PIECE * 128;                // one slot's term of a piece
+constexpr uint32_t RING = 3 * 2 * SUB;               // a piece: 3 terms x 2 slots
+constexpr uint32_t OFF_R = OFF_S + 2 * PANEL;        // 2 pieces
+constexpr uint32_t OFF_GATE = OFF_R + 2 * RING;      // 2 buffers x 2 slots x Gates
+constexpr uint32_t GATE_BYTES = 4 * CH * 4;
+constexpr uint32_t OFF_MISC = OFF_GATE + 4 * GATE_BYTES;
+constexpr uint32_t MISC_SUMS = 0;                    // block sums [2 buffers][2 slots][4]
+constexpr uint32_t MISC_BAR = 64;
+constexpr uint32_t MISC_TMEM = 320;
+constexpr uint32_t MISC_SEG = 324;                   // sequence, segment in it, count, first, begin, length
+constexpr uint32_t MISC_BYTES = 384;
+constexpr uint32_t CHUNK_SMEM = OFF_MISC + MISC_BYTES + 1024;
+static_assert(CHUNK_SMEM <= 232448, "exceeds the 227 KB per-block shared memory limit");
+
+// Gates of one slot and chunk (floats): prefix sums of a inside each 32-block, d, h_j = 2^{sum of a
+// behind j in its block} d_j, w_j = 2^{sum of a behind j in the chunk} d_j.
+constexpr int GT_C = 0, GT_D = CH, GT_H = 2 * CH, GT_W = 3 * CH;
+
+// ---- TMEM columns (all 128 lanes)
+constexpr uint32_t TM_G = 0;     // G fp32 [token i][token j]
+constexpr uint32_t TM_M = 128;   // M bf16 pairs, 64 columns per slot
+constexpr uint32_t TM_Y = 256;   // y fp32 [token][slot, channel]
+constexpr uint32_t TM_ST = 384;  // S^T fp32 [state][slot, channel]
+
+// Barriers. *F full, *E empty.
+enum {
+    B_XF = 0, B_XE = 2, B_BF = 4, B_BE = 6, B_CF = 8,
+    B_GF = 9,   // G in TMEM
+    B_ID = 10,  // inter product done (y's columns written, C tile free)
+    B_MR = 11,  // M written, y scaled, G read
+    B_YD = 12,  // intra product done
+    B_YF = 13,  // y's columns read
+    B_SC = 14,  // state operand written and state decayed
+    B_SD = 15,  // state product done
+    B_RF = 16, B_RE = 18,  // ring of X' pieces
+    B_PF = 20, B_PE = 22,  // gates
+    B_YS = 24,             // output tile written, per slot
+    B_DR = 26,             // every MMA done (exit)
+    NBARS = 27
+};
+static_assert(MISC_BAR + 8 * NBARS <= MISC_TMEM, "barriers overlap the TMEM address word");
+
+struct ChunkParams {
+    CUtensorMap tm_x, tm_b, tm_c, tm_y;
+    ScanArgs a;
+    float4* part;      // state pass: final states of segments, [segment][unit][slot][channel / 4][state]
+    float* part_log;   // and their log2 decays, [segment][unit][slot]
+    unsigned int* status;
+    int ptiles;        // slots per head
+    int pairs;         // slot pairs per group
+    int units;         // G * pairs
+    int seg_tokens;    // tokens per segment (a multiple of 128), 0: one segment per sequence
+};
+
+__device__ __noinline__ void scan_wait_failed(unsigned int* status) { atomicOr(status, 1u | (1u << 16)); }
+
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t top_halves(float a, float b) {  // bf16 pair of the leading halves
+    return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+}
+__device__ __forceinline__ float head(float a) { return __uint_as_float(__float_as_uint(a) & 0xFFFF0000u); }
+
+// kState: the state pass of a segmented call: every segment but a sequence's last from a zero state;
+// its final state and log decay go to part / part_log, no output.
+template <bool kState>
+__global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __grid_constant__ ChunkParams p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sb = ptx::smem_u32(smem);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const ScanArgs& a = p.a;
+    volatile int* seg = reinterpret_cast<volatile int*>(smem + OFF_MISC + MISC_SEG);
+    const uint32_t bar0 = sb + OFF_MISC + MISC_BAR;
+    auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
+
+    // ---- this CTA's segment ----
+    const int unit = blockIdx.x % p.units, sid = blockIdx.x / p.units;
+    if (warp == 0) {
+        int seq = sid, j = 0, first = sid, count = 1;
+        if (p.seg_tokens > 0 && a.cu == nullptr) {
+            count = max(1, (a.T + p.seg_tokens - 1) / p.seg_tokens);
+            seq = sid / count;
+            first = seq * count;
+            j = sid - first;
+        } else if (p.seg_tokens > 0) {  // packed: segments in the order of the sequences
+            int base = 0;
+            seq = a.N;
+            for (int s0 = 0; s0 < a.N; s0 += 32) {
+                int n = 0;
+                if (s0 + lane < a.N) {
+                    int64_t b, e;
+                    seq_range(a.cu, s0 + lane, a.T, b, e);
+                    n = max(1, (int)((e - b + p.seg_tokens - 1) / p.seg_tokens));
+                }
+                int inc = n;
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) {
+                    const int t = __shfl_up_sync(0xffffffffu, inc, off);
+                    if (lane >= off) inc += t;
+                }
+                const unsigned hit = __ballot_sync(0xffffffffu, base + inc > sid);
+                if (hit) {
+                    const int src = __ffs(hit) - 1;
+                    seq = s0 + src;
+                    count = __shfl_sync(0xffffffffu, n, src);
+                    first = base + __shfl_sync(0xffffffffu, inc, src) - count;
+                    j = sid - first;
+                    break;
+                }
+                base += __shfl_sync(0xffffffffu, inc, 31);
+            }
+        }
+        if (lane == 0) {
+            int64_t b = 0, e = 0;
+            if (seq < a.N) seq_range(a.cu, seq, a.T, b, e);
+            // rows fit 31 bits (checked by the launcher)
+            const int begin = (int)b + j * p.seg_tokens;
+            seg[0] = seq;
+            seg[1] = j;
+            seg[2] = count;
+            seg[3] = first;
+            seg[4] = begin;
+            seg[5] = (p.seg_tokens > 0) ? min(p.seg_tokens, (int)e - begin) : (int)(e - b);
+        }
+    }
+    if (tid == 32) {
+        for (int i = 0; i < NBARS; ++i) {
+            int n = 1;
+            if (i == B_MR || i == B_YF || i == B_SC || i == B_RF || i == B_RF + 1) n = 8;
+            if (i == B_PE || i == B_PE + 1) n = kState ? 8 : 16;
+            if (i == B_XE || i == B_XE + 1) n = kState ? 8 : 1;
+            if (i == B_YS || i == B_YS + 1) n = 4;
+            ptx::mbar_init(bar(i), n);
+        }
+        ptx::fence_mbar_init();
+    }
+    if (warp == 16) {
+        ptx::tmem_alloc(sb + OFF_MISC + MISC_TMEM, 512);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + OFF_MISC + MISC_TMEM);
+    const int seq = seg[0], seg_j = seg[1], seg_count = seg[2], seg_first = seg[3];
+    const int row0 = seg[4], len = seg[5];
+    // no such segment (the grid covers the most there can be); the state pass skips last segments
+    const bool idle = seq >= a.N || (kState && seg_j == seg_count - 1);
+    const int nc = idle ? 0 : (len + CH - 1) / CH;
+
+    // ---- slots: head and channel tile ----
+    const int g = unit / p.pairs, r_heads = a.H / a.G;
+    const int slot0 = 2 * (unit - g * p.pairs), nslots = r_heads * p.ptiles;
+    const bool second = slot0 + 1 < nslots;  // an odd one out runs its slot twice and stores it once
+    auto slot_head = [&](int s) { return g * r_heads + (slot0 + (second ? s : 0)) / p.ptiles; };
+    auto slot_tile = [&](int s) { return (slot0 + (second ? s : 0)) % p.ptiles; };
+    const int npanel = a.NS > 64 ? 2 : 1;
+
+    // Waits are bounded; the vote keeps a warp together when one runs out.
+    auto wait = [&](int b, uint32_t parity) -> bool {
+        const bool ok = ptx::mbar_wait(bar(b), parity & 1u, WAIT_ITERS);
+        if (!ok) scan_wait_failed(p.status);
+        return ok;
+    };
+    auto warp_wait = [&](int b, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(b, parity)); };
+    auto warp_arrive = [&](int b) {
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar(b));
+    };
+    float* sums = reinterpret_cast<float*>(smem + OFF_MISC + MISC_SUMS);
+    auto gates = [&](int buf, int s) { return reinterpret_cast<float*>(smem + OFF_GATE + (2 * buf + s) * GATE_BYTES); };
+    const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16);  // this warp's TMEM lane quarter
+
+    if (warp < 8) {
+        // ================= M, the scaling of y, the output tile =================
+        if constexpr (!kState) {
+            const int s = warp >> 2, q = warp & 3, i = 32 * q + lane;
+            const uint32_t tm_m = tl + TM_M + 64 * s, tm_y = tl + TM_Y + 64 * s;
+            const int h = slot_head(s), c0 = slot_tile(s) * TILE;
+            const float D = a.D ? a.D[h] : 0.f;
+            const bool stores = s == 0 || second;
+            if (nc > 0) {  // blocks right of the diagonal stay zero
+                const uint32_t zero[16] = {};
+                for (int b = q + 1; b < 4; ++b) ptx::tmem_st16(tm_m + 16 * b, zero);
+            }
+            auto body = [&](int k) -> bool {
+                const int buf = k & 1;
+                const uint32_t m = (uint32_t)k >> 1;
+                if (!warp_wait(B_PF + buf, m) || !warp_wait(B_GF, k)) return false;
+                ptx::tc_fence_after();
+                const float* gt = gates(buf, s);
+                const float ci = gt[GT_C + i];
+                const float* R = sums + (2 * buf + s) * 4;
+                float before = 0.f;  // sum of a over the blocks between block b and this row's
+                float rowsum[4];
+#pragma unroll
+                for (int b = 3; b >= 0; --b) {
+                    rowsum[b] = before;
+                    if (b < q) before += R[b];
+                }
+#pragma unroll 1
+                for (int b = 0; b < q; ++b) {
+                    float v[32];
+                    ptx::tmem_ld32(tl + TM_G + 32 * b, v);
+                    const float f = ex2f(ci + (b == 0 ? rowsum[0] : b == 1 ? rowsum[1] : rowsum[2]));
+                    const uint64_t ff = f2_pack(f, f);
+                    uint32_t o[16];
+                    ptx::tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 h4 = ld4(gt + GT_H + 32 * b + j);
+                        float x0, x1;
+                        f2_unpack(f2_mul(f2_mul(f2_pack(h4.x, h4.y), ff), f2_pack(v[j], v[j + 1])), x0, x1);
+                        o[j / 2] = pack_bf16(x0, x1);
+                        f2_unpack(f2_mul(f2_mul(f2_pack(h4.z, h4.w), ff), f2_pack(v[j + 2], v[j + 3])), x0, x1);
+                        o[j / 2 + 1] = pack_bf16(x0, x1);
+                    }
+                    ptx::tmem_st16(tm_m + 16 * b, o);
+                }
+                {
+                    float v[32];
+                    ptx::tmem_ld32(tl + TM_G + 32 * q, v);
+                    uint32_t o[16];
+                    ptx::tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 c4 = ld4(gt + GT_C + 32 * q + j), d4 = ld4(gt + GT_D + 32 * q + j);
+                        // a select, not a product with zero: rows behind a sequence may hold anything
+                        const float x0 = j + 0 <= lane ? v[j + 0] * (ex2f(ci - c4.x) * d4.x) : 0.f;
+                        const float x1 = j + 1 <= lane ? v[j + 1] * (ex2f(ci - c4.y) * d4.y) : 0.f;
+                        const float x2 = j + 2 <= lane ? v[j + 2] * (ex2f(ci - c4.z) * d4.z) : 0.f;
+                        const float x3 = j + 3 <= lane ? v[j + 3] * (ex2f(ci - c4.w) * d4.w) : 0.f;
+                        o[j / 2] = pack_bf16(x0, x1);
+                        o[j / 2 + 1] = pack_bf16(x2, x3);
+                    }
+                    ptx::tmem_st16(tm_m + 16 * q, o);
+                }
+                // Y <- e^{c_i} (C S^T), so that M X accumulates onto it
+                const float e = ex2f(ci + before);
+                const uint64_t ee = f2_pack(e, e);
+                if (!warp_wait(B_ID, k)) return false;
+                ptx::tc_fence_after();
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    float v[32];
+                    uint32_t o[32];
+                    ptx::tmem_ld32(tm_y + 32 * hf, v);
+                    ptx::tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        float x0, x1;
+                        f2_unpack(f2_mul(f2_pack(v[j], v[j + 1]), ee), x0, x1);
+                        o[j] = __float_as_uint(x0);
+                        o[j + 1] = __float_as_uint(x1);
+                    }
+                    ptx::tmem_st32(tm_y + 32 * hf, o);
+                }
+                ptx::tmem_wait_st();
+                ptx::tc_fence_before();
+                warp_arrive(B_MR);
+                if (lane == 0) ptx::mbar_arrive(bar(B_PE + buf));
+                // ---- output tile: y = Y + D x, in place of x ----
+                if (!warp_wait(B_XF + buf, m) || !warp_wait(B_YD, k)) return false;
+                ptx::tc_fence_after();
+                const uint32_t xt = sb + OFF_X + (2 * buf + s) * PANEL;
+                const uint64_t dd = f2_pack(D, D);
+                const int valid = min(CH, len - CH * k);
+                const int64_t row = (int64_t)row0 + CH * k + i;
+                __nv_bfloat16* yr = a.y + (row * a.H + h) * a.P + c0;
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    float v[32];
+                    ptx::tmem_ld32(tm_y + 32 * hf, v);
+                    ptx::tmem_wait_ld();
+                    if (hf == 1) {
+                        ptx::tc_fence_before();
+                        warp_arrive(B_YF);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const uint32_t at = xt + sw_chunk(i, 4 * hf + c, CH);
+                        uint32_t u[4];
+                        ld_shared_v4(at, u[0], u[1], u[2], u[3]);
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) {
+                            float x0, x1;
+                            f2_unpack(f2_fma(f2_pack(__uint_as_float(u[t] << 16), __uint_as_float(u[t] & 0xFFFF0000u)), dd,
+                                             f2_pack(v[8 * c + 2 * t], v[8 * c + 2 * t + 1])),
+                                      x0, x1);
+                            u[t] = pack_bf16(x0, x1);
+                        }
+                        if (valid == CH) {
+                            st_shared_v4(at, u[0], u[1], u[2], u[3]);
+                        } else if (stores && i < valid && c0 + 32 * hf + 8 * c < a.P) {
+                            *reinterpret_cast<uint4*>(yr + 32 * hf + 8 * c) = make_uint4(u[0], u[1], u[2], u[3]);
+                        }
+                    }
+                }
+                if (valid == CH) {
+                    ptx::fence_proxy_async_smem();
+                    warp_arrive(B_YS + s);
+                }
+                return true;
+            };
+            for (int k = 0; k < nc; ++k)
+                if (!body(k)) break;
+        }
+    } else if (warp < 16) {
+        // ================= X' and the state =================
+        const int s = (warp >> 2) - 2, n = 32 * (warp & 3) + lane;
+        const int t128 = tid & 127, pt = t128 >> 3, pc = t128 & 7;  // token and 16-byte chunk of a piece
+        const uint32_t tm_s = tl + TM_ST + 64 * s;
+        const int h = slot_head(s), c0 = slot_tile(s) * TILE;
+        const bool stores = s == 0 || second;
+        const size_t sbase = (((size_t)(seq < a.N ? seq : 0) * a.H + h) * a.P + c0) * a.NS + n;
+        bool ok = !idle;
+        if (ok) {  // entry state: the initial state carried through the earlier segments
+#pragma unroll 1
+            for (int hf = 0; hf < 2; ++hf) {
+                float v[32];
+#pragma unroll
+                for (int c = 0; c < 32; ++c) {
+                    const int ch = 32 * hf + c;
+                    v[c] = (!kState && a.s0 != nullptr && c0 + ch < a.P && n < a.NS) ? a.s0[sbase + (size_t)ch * a.NS] : 0.f;
+                }
+                if constexpr (!kState) {
+                    for (int e = seg_first; e < seg_first + seg_j; ++e) {
+                        const size_t at = ((size_t)e * p.units + unit) * 2 + s;
+                        const float decay = ex2f(p.part_log[at]);
+                        const float4* src = p.part + (at * (TILE / 4) + 8 * hf) * CH + n;
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            const float4 f = src[c * CH];
+                            v[4 * c] = fmaf(decay, v[4 * c], f.x);
+                            v[4 * c + 1] = fmaf(decay, v[4 * c + 1], f.y);
+                            v[4 * c + 2] = fmaf(decay, v[4 * c + 2], f.z);
+                            v[4 * c + 3] = fmaf(decay, v[4 * c + 3], f.w);
+                        }
+                    }
+                }
+                uint32_t o[32];
+#pragma unroll
+                for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(v[c]);
+                ptx::tmem_st32(tm_s + 32 * hf, o);
+            }
+            ptx::tmem_wait_st();
+        }
+        float log_decay = 0.f;
+        // piece i of chunk k: 16 tokens x 64 channels of X' = w x as three bf16 terms
+        auto piece = [&](int k, int i, int valid, const float* gt) -> bool {
+            const uint32_t use = (uint32_t)(PIECES * k + i) >> 1, slot = (uint32_t)i & 1u;
+            if (use > 0 && !warp_wait(B_RE + slot, use - 1)) return false;
+            const int t = PIECE * i + pt;
+            const float w = gt[GT_W + t];
+            const uint64_t ww = f2_pack(w, w);
+            uint32_t u[4], hi[4], mid[4], lo[4];
+            ld_shared_v4(sb + OFF_X + (2 * (k & 1) + s) * PANEL + sw_chunk(t, pc, CH), u[0], u[1], u[2], u[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t x = t < valid ? u[e] : 0u;
+                const uint64_t v = f2_mul(f2_pack(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u)), ww);
+                float v0, v1, r0, r1, l0, l1;
+                f2_unpack(v, v0, v1);
+                hi[e] = top_halves(v0, v1);
+                const uint64_t r = f2_sub(v, f2_pack(head(v0), head(v1)));
+                f2_unpack(r, r0, r1);
+                mid[e] = top_halves(r0, r1);
+                f2_unpack(f2_sub(r, f2_pack(head(r0), head(r1))), l0, l1);
+                lo[e] = top_halves(l0, l1);
+            }
+            const uint32_t at = sb + OFF_R + slot * RING + s * SUB + sw_chunk(pt, pc, PIECE);
+            st_shared_v4(at, hi[0], hi[1], hi[2], hi[3]);
+            st_shared_v4(at + 2 * SUB, mid[0], mid[1], mid[2], mid[3]);
+            st_shared_v4(at + 4 * SUB, lo[0], lo[1], lo[2], lo[3]);
+            ptx::fence_proxy_async_smem();
+            warp_arrive(B_RF + slot);
+            return true;
+        };
+        auto body = [&](int k) -> bool {
+            const int buf = k & 1;
+            const uint32_t m = (uint32_t)k >> 1;
+            const int valid = min(CH, len - CH * k);
+            if (!warp_wait(B_PF + buf, m) || !warp_wait(B_XF + buf, m)) return false;
+            if (valid < CH) {
+                // the rows behind the sequence belong to others and may hold anything: zeros in X and B,
+                // whose products would otherwise reach valid rows as 0 x NaN
+                if (!warp_wait(B_BF + buf, m)) return false;
+                for (int e = t128; e < (CH - valid) * 8; e += 128) {
+                    const uint32_t off = sw_chunk(valid + (e >> 3), e & 7, CH);
+                    st_shared_v4(sb + OFF_X + (2 * buf + s) * PANEL + off, 0, 0, 0, 0);
+                    if (s < npanel) st_shared_v4(sb + OFF_B + (2 * buf + s) * PANEL + off, 0, 0, 0, 0);
+                }
+                ptx::fence_proxy_async_smem();
+            }
+            const float* gt = gates(buf, s);
+            if (!piece(k, 0, valid, gt) || !piece(k, 1, valid, gt)) return false;
+            // the state: bf16 copy as the operand of C S^T, and its decay over this chunk
+            if (k > 0 && !warp_wait(B_SD, k - 1)) return false;
+            ptx::tc_fence_after();
+            const float* R = sums + (2 * buf + s) * 4;
+            const float total = (R[0] + R[1]) + (R[2] + R[3]);
+            log_decay += total;
+            const float decay = ex2f(total);
+            const uint64_t dd = f2_pack(decay, decay);
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                float v[32];
+                uint32_t o[32];
+                ptx::tmem_ld32(tm_s + 32 * hf, v);
+                ptx::tmem_wait_ld();
+                if constexpr (!kState) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        st_shared_v4(sb + OFF_S + s * PANEL + sw_chunk(n, 4 * hf + c, CH), pack_bf16(v[8 * c], v[8 * c + 1]),
+                                     pack_bf16(v[8 * c + 2], v[8 * c + 3]), pack_bf16(v[8 * c + 4], v[8 * c + 5]),
+                                     pack_bf16(v[8 * c + 6], v[8 * c + 7]));
+                }
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) {
+                    float x0, x1;
+                    f2_unpack(f2_mul(f2_pack(v[j], v[j + 1]), dd), x0, x1);
+                    o[j] = __float_as_uint(x0);
+                    o[j + 1] = __float_as_uint(x1);
+                }
+                ptx::tmem_st32(tm_s + 32 * hf, o);
+            }
+            ptx::tmem_wait_st();
+            ptx::fence_proxy_async_smem();
+            ptx::tc_fence_before();
+            warp_arrive(B_SC);
+#pragma unroll 1
+            for (int i = 2; i < PIECES; ++i)
+                if (!piece(k, i, valid, gt)) return false;
+            warp_arrive(B_PE + buf);
+            if (kState) warp_arrive(B_XE + buf);
+            return true;
+        };
+        for (int k = 0; ok && k < nc; ++k) ok = body(k);
+        if (ok && nc > 0) {
+            ok = warp_wait(B_SD, nc - 1);
+            ptx::tc_fence_after();
+        }
+        if (ok && (kState || seg_j == seg_count - 1)) {
+            const size_t at = ((size_t)sid * p.units + unit) * 2 + s;
+            if (kState && n == 0) p.part_log[at] = log_decay;
+#pragma unroll 1
+            for (int hf = 0; hf < 2; ++hf) {
+                float v[32];
+                ptx::tmem_ld32(tm_s + 32 * hf, v);
+                ptx::tmem_wait_ld();
+                if (kState) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        p.part[(at * (TILE / 4) + 8 * hf + c) * CH + n] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+                } else if (stores && n < a.NS) {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (c0 + 32 * hf + c < a.P) a.sf[sbase + (size_t)(32 * hf + c) * a.NS] = v[c];
+                }
+            }
+        }
+    } else if (warp == 16) {
+        // ================= MMA issue (one thread) =================
+        if (lane == 0) {
+            constexpr uint32_t ID_G = ptx::idesc_bf16(128, 128, 0, 0, 0);      // C B^T
+            constexpr uint32_t ID_INTER = ptx::idesc_bf16(128, 128, 0, 1, 0);  // C S^T       (B MN-major)
+            constexpr uint32_t ID_STATE = ptx::idesc_bf16(128, 128, 1, 1, 0);  // B^T X'      (both MN-major)
+            constexpr uint32_t ID_INTRA = ptx::idesc_bf16(128, 64, 0, 1, 0);   // M X         (A in TMEM, B MN-major)
+            const uint32_t d16 = ptx::sw128_desc_lo(sb, 16), dpanel = ptx::sw128_desc_lo(sb, PANEL), dsub = ptx::sw128_desc_lo(sb, SUB);
+            auto desc = [](uint32_t base, uint32_t off) { return ptx::desc_pair(base + (off >> 4), ptx::sw128_desc_hi(1024)); };
+            auto kmajor = [](int st) { return (uint32_t)(st >> 2) * PANEL + (uint32_t)(st & 3) * 32u; };
+            const int ks = (a.NS + 15) / 16;  // K steps over the state dimension
+            auto issue_g = [&](int k) -> bool {
+                if (!wait(B_BF + (k & 1), (uint32_t)k >> 1) || !wait(B_CF, k)) return false;
+                ptx::tc_fence_after();
+                for (int st = 0; st < ks; ++st)
+                    ptx::mma_bf16(tmem + TM_G, desc(d16, OFF_C + kmajor(st)), desc(d16, OFF_B + (k & 1) * 2 * PANEL + kmajor(st)), ID_G, st > 0);
+                ptx::mma_commit(bar(B_GF));
+                return true;
+            };
+            auto body = [&](int k) -> bool {
+                const int buf = k & 1;
+                if (kState) {
+                    if (!wait(B_BF + buf, (uint32_t)k >> 1)) return false;
+                }
+                if (!wait(B_SC, k)) return false;
+                if constexpr (!kState) {
+                    if (k > 0 && !wait(B_YF, k - 1)) return false;
+                    ptx::tc_fence_after();
+                    for (int st = 0; st < ks; ++st)
+                        ptx::mma_bf16(tmem + TM_Y, desc(d16, OFF_C + kmajor(st)), desc(dpanel, OFF_S + st * 2048u), ID_INTER, st > 0);
+                    ptx::mma_commit(bar(B_ID));
+                }
+                ptx::tc_fence_after();
+                for (int i = 0; i < PIECES; ++i) {
+                    const uint32_t use = (uint32_t)(PIECES * k + i) >> 1, slot = (uint32_t)i & 1u;
+                    if (!wait(B_RF + slot, use)) return false;
+                    ptx::tc_fence_after();
+                    const uint64_t ad = desc(dpanel, OFF_B + buf * 2 * PANEL + i * 2048u);
+#pragma unroll
+                    for (int term = 0; term < 3; ++term)
+                        ptx::mma_bf16(tmem + TM_ST, ad, desc(dsub, OFF_R + slot * RING + term * 2 * SUB), ID_STATE, 1);
+                    ptx::mma_commit(bar(B_RE + slot));
+                }
+                ptx::mma_commit(bar(B_SD));
+                ptx::mma_commit(bar(B_BE + buf));
+                if constexpr (!kState) {
+                    if (!wait(B_MR, k)) return false;
+                    ptx::tc_fence_after();
+#pragma unroll
+                    for (int s = 0; s < 2; ++s)
+#pragma unroll
+                        for (int st = 0; st < PIECES; ++st)
+                            ptx::mma_bf16_ts(tmem + TM_Y + 64 * s, tmem + TM_M + 64 * s + 8 * st,
+                                             desc(d16, OFF_X + (2 * buf + s) * PANEL + st * 2048u), ID_INTRA, 1);
+                    ptx::mma_commit(bar(B_YD));
+                    if (k + 1 < nc && !issue_g(k + 1)) return false;
+                }
+                return true;
+            };
+            bool ok = true;
+            if (!kState && nc > 0) ok = issue_g(0);
+            for (int k = 0; ok && k < nc; ++k) ok = body(k);
+            ptx::mma_commit(bar(B_DR));  // nothing in flight when the CTA leaves
+            wait(B_DR, 0);
+        }
+        __syncwarp();
+    } else if (warp == 17) {
+        // ================= TMA loads (one thread) =================
+        if (lane == 0) {
+            ptx::prefetch_tensormap(&p.tm_x);
+            ptx::prefetch_tensormap(&p.tm_b);
+            if (!kState) ptx::prefetch_tensormap(&p.tm_c);
+            const int h0 = slot_head(0), h1 = slot_head(1), t0 = slot_tile(0) * TILE, t1 = slot_tile(1) * TILE;
+            int nb = 0, nx = 0, ncl = 0;  // loads issued
+            auto body = [&](int k) -> bool {
+                const int buf = k & 1, row = row0 + CH * k;
+                const uint32_t m = (uint32_t)k >> 1;
+                if (m > 0 && !wait(B_BE + buf, m - 1)) return false;
+                ++nb;
+                ptx::mbar_arrive_expect_tx(bar(B_BF + buf), npanel * PANEL);
+                for (int c = 0; c < npanel; ++c)
+                    ptx::tma_load_4d(sb + OFF_B + (2 * buf + c) * PANEL, &p.tm_b, bar(B_BF + buf), 64 * c, g, row, 0);
+                if (!kState && k == 0) {
+                    ++ncl;
+                    ptx::mbar_arrive_expect_tx(bar(B_CF), npanel * PANEL);
+                    for (int c = 0; c < npanel; ++c) ptx::tma_load_4d(sb + OFF_C + c * PANEL, &p.tm_c, bar(B_CF), 64 * c, g, row, 0);
+                }
+                if (m > 0 && !wait(B_XE + buf, m - 1)) return false;
+                ++nx;
+                ptx::mbar_arrive_expect_tx(bar(B_XF + buf), 2 * PANEL);
+                ptx::tma_load_4d(sb + OFF_X + 2 * buf * PANEL, &p.tm_x, bar(B_XF + buf), t0, h0, row, 0);
+                ptx::tma_load_4d(sb + OFF_X + (2 * buf + 1) * PANEL, &p.tm_x, bar(B_XF + buf), t1, h1, row, 0);
+                if (!kState && k > 0) {
+                    if (!wait(B_ID, k - 1)) return false;
+                    ++ncl;
+                    ptx::mbar_arrive_expect_tx(bar(B_CF), npanel * PANEL);
+                    for (int c = 0; c < npanel; ++c) ptx::tma_load_4d(sb + OFF_C + c * PANEL, &p.tm_c, bar(B_CF), 64 * c, g, row, 0);
+                }
+                return true;
+            };
+            for (int k = 0; k < nc; ++k)
+                if (!body(k)) break;
+            // no load in flight when the CTA leaves
+            for (int buf = 0; buf < 2; ++buf) {
+                if (nb > buf) wait(B_BF + buf, (uint32_t)(nb - 1 - buf) >> 1);
+                if (nx > buf) wait(B_XF + buf, (uint32_t)(nx - 1 - buf) >> 1);
+            }
+            if (ncl > 0) wait(B_CF, (uint32_t)(ncl - 1));
+        }
+        __syncwarp();
+    } else if (warp == 18) {
+        // ================= gates of both slots =================
+        float A2[2], bias[2], next[2][4];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            A2[s] = a.A[slot_head(s)] * LOG2E;
+            bias[s] = a.dt_bias ? a.dt_bias[slot_head(s)] : 0.f;
+        }
+        auto load = [&](int k) {  // clamped to the segment's rows
+            const int last = len - 1 - CH * k;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) next[s][i] = scan_dt(a, (int64_t)row0 + CH * k + min(4 * lane + i, last), slot_head(s));
+        };
+        auto body = [&](int k) -> bool {
+            const int buf = k & 1, valid = len - CH * k;
+            float d[2][4];
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float v = next[s][i] + bias[s];
+                    if (a.softplus) v = softplus(v);
+                    d[s][i] = 4 * lane + i < valid ? v : 0.f;
+                }
+            if (k + 1 < nc) load(k + 1);
+            if (k >= 2 && !warp_wait(B_PE + buf, ((uint32_t)k >> 1) - 1)) return false;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                // log2 decays; the clamp keeps sums of 128 finite, and 2^-1e30 is zero as well
+                float t[4], pre[4], suf[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) t[i] = fmaxf(d[s][i] * A2[s], -1e30f);
+                pre[0] = t[0], pre[1] = t[0] + t[1], pre[2] = pre[1] + t[2], pre[3] = pre[2] + t[3];
+                suf[3] = 0.f, suf[2] = t[3], suf[1] = t[3] + t[2], suf[0] = suf[1] + t[1];
+                // sums over the 8 lanes of a 32-token block, from the left and, for the accuracy of the
+                // short distances, from the right
+                float inc = pre[3], dec = pre[3];
+#pragma unroll
+                for (int off = 1; off < 8; off <<= 1) {
+                    const float u = __shfl_up_sync(0xffffffffu, inc, off, 8), v = __shfl_down_sync(0xffffffffu, dec, off, 8);
+                    if ((lane & 7) >= off) inc += u;
+                    if ((lane & 7) + off < 8) dec += v;
+                }
+                float left = __shfl_up_sync(0xffffffffu, inc, 1, 8), right = __shfl_down_sync(0xffffffffu, dec, 1, 8);
+                if ((lane & 7) == 0) left = 0.f;
+                if ((lane & 7) == 7) right = 0.f;
+                float R[4];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) R[b] = __shfl_sync(0xffffffffu, inc, 8 * b + 7);
+                float behind = 0.f;
+#pragma unroll
+                for (int b = 3; b > 0; --b)
+                    if (b > (lane >> 3)) behind += R[b];
+                const float f = ex2f(behind);
+                float hv[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) hv[i] = ex2f(right + suf[i]) * d[s][i];
+                float* gt = gates(buf, s) + 4 * lane;
+                *reinterpret_cast<float4*>(gt + GT_C) = make_float4(left + pre[0], left + pre[1], left + pre[2], left + pre[3]);
+                *reinterpret_cast<float4*>(gt + GT_D) = make_float4(d[s][0], d[s][1], d[s][2], d[s][3]);
+                *reinterpret_cast<float4*>(gt + GT_H) = make_float4(hv[0], hv[1], hv[2], hv[3]);
+                *reinterpret_cast<float4*>(gt + GT_W) = make_float4(hv[0] * f, hv[1] * f, hv[2] * f, hv[3] * f);
+                if (lane == 0) *reinterpret_cast<float4*>(sums + (2 * buf + s) * 4) = make_float4(R[0], R[1], R[2], R[3]);
+            }
+            warp_arrive(B_PF + buf);
+            return true;
+        };
+        if (nc > 0) load(0);
+        for (int k = 0; k < nc; ++k)
+            if (!body(k)) break;
+    } else {
+        // ================= TMA stores of full output tiles (one thread) =================
+        if (!kState && lane == 0) {
+            const int h0 = slot_head(0), h1 = slot_head(1), t0 = slot_tile(0) * TILE, t1 = slot_tile(1) * TILE;
+            for (int k = 0; k < nc && len - CH * k >= CH; ++k) {
+                const int buf = k & 1, row = row0 + CH * k;
+                if (!wait(B_YS, k)) break;
+                tma_store_4d(&p.tm_y, sb + OFF_X + 2 * buf * PANEL, t0, h0, row, 0);
+                if (!wait(B_YS + 1, k)) break;
+                if (second) tma_store_4d(&p.tm_y, sb + OFF_X + (2 * buf + 1) * PANEL, t1, h1, row, 0);
+                ptx::bulk_wait_read_all();
+                ptx::mbar_arrive(bar(B_XE + buf));
+            }
+            ptx::bulk_wait_all();
+        }
+        __syncwarp();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    if (warp == 16) ptx::tmem_dealloc(tmem, 512);
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeFn encode_fn() {
+    static std::once_flag once;
+    static EncodeFn fn = nullptr;
+    std::call_once(once, []() {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult qres;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) == cudaSuccess &&
+            qres == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeFn>(ptr);
+    });
+    return fn;
+}
+
+// bf16 [rows][units][width] with a row stride; box 64 x 1 x 128 rows, 128-byte swizzle, zeros outside.
+static bool row_map(CUtensorMap* m, const void* base, int width, int units, int64_t rows, int64_t stride) {
+    EncodeFn enc = encode_fn();
+    if (!enc) return false;
+    cuuint64_t dims[4] = {(cuuint64_t)width, (cuuint64_t)units, (cuuint64_t)rows, 1};
+    cuuint64_t strides[3] = {(cuuint64_t)width * 2, (cuuint64_t)stride * 2, (cuuint64_t)stride * 2 * (cuuint64_t)rows};
+    cuuint32_t box[4] = {64, 1, CH, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+static cudaError_t chunk_smem_attr() {
+    static std::atomic<uint64_t> done_mask{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = (dev < 64) ? (1ull << dev) : 0;
+    if (bit && (done_mask.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    for (auto fn : {scan_chunk_kernel<false>, scan_chunk_kernel<true>}) {
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)CHUNK_SMEM);
+        if (e != cudaSuccess) return e;
+    }
+    if (bit) done_mask.fetch_or(bit, std::memory_order_acq_rel);
+    return cudaSuccess;
+}
+
+ChunkPlan plan_scan_chunks(int N, int T, bool packed, int H, int P, int G, int sms) {
+    ChunkPlan pl{};
+    const int ptiles = (P + TILE - 1) / TILE;
+    pl.pairs = (H / G * ptiles + 1) / 2;
+    pl.units = G * pl.pairs;
+    pl.segments = N;
+    const int64_t rows = packed ? T : (int64_t)N * T;
+    const int64_t chunks = N > 0 ? (rows / N + CH - 1) / CH : 0;  // of the mean sequence
+    // Wave model. Measured on B200: an output pass takes about 1.8 us per chunk and pair and a state pass
+    // 1.1, a CTA's start and end about 5 us, the second launch 3 us. Segments pay where the
+    // (sequence, pair) units alone leave SMs idle.
+    auto waves = [&](int64_t ctas) { return (double)((ctas + sms - 1) / sms); };
+    double best = waves((int64_t)N * pl.units) * (1.8 * chunks + 5.0);
+    for (int64_t s = 2; s <= chunks && s <= 64 && (int64_t)N * pl.units * (s - 1) < sms; ++s) {
+        const int64_t per = (chunks + s - 1) / s, cut = (chunks + per - 1) / per;
+        if (cut < 2) continue;
+        const double t = waves((int64_t)N * pl.units * cut) * (1.8 * per + 5.0 + 0.4 * cut) +
+                         waves((int64_t)N * pl.units * (cut - 1)) * (1.1 * per + 5.0) + 3.0;
+        if (t < best) {
+            best = t;
+            pl.seg_tokens = (int)(per * CH);
+            pl.segments = packed ? (int64_t)T / pl.seg_tokens + N : (int64_t)N * ((T + pl.seg_tokens - 1) / pl.seg_tokens);
+        }
+    }
+    const int64_t parts = pl.seg_tokens > 0 ? pl.segments * pl.units * 2 : 0;
+    pl.part_bytes = (size_t)parts * TILE * CH * 4;
+    pl.log_bytes = ((size_t)parts * 4 + 255) / 256 * 256;
+    return pl;
+}
+
+cudaError_t launch_scan_chunks(const ScanArgs& a, const ChunkPlan& pl, int64_t rows, void* workspace, void* scratch,
+                               cudaStream_t stream) {
+    ChunkParams p;
+    memset(&p, 0, sizeof(p));
+    if (!row_map(&p.tm_x, a.x, a.P, a.H, rows, a.xs) || !row_map(&p.tm_b, a.B, a.NS, a.G, rows, a.bs) ||
+        !row_map(&p.tm_c, a.C, a.NS, a.G, rows, a.cs) || !row_map(&p.tm_y, a.y, a.P, a.H, rows, (int64_t)a.H * a.P))
+        return cudaErrorInvalidValue;
+    cudaError_t e = chunk_smem_attr();
+    if (e != cudaSuccess) return e;
+    p.a = a;
+    p.status = static_cast<unsigned int*>(workspace);
+    p.part_log = static_cast<float*>(scratch);
+    p.part = reinterpret_cast<float4*>(static_cast<uint8_t*>(scratch) + pl.log_bytes);
+    p.ptiles = (a.P + TILE - 1) / TILE;
+    p.pairs = pl.pairs;
+    p.units = pl.units;
+    p.seg_tokens = pl.seg_tokens;
+    const int64_t ctas = pl.segments * pl.units;
+    if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
+    if (pl.seg_tokens > 0) {
+        scan_chunk_kernel<true><<<(unsigned)ctas, CHUNK_THREADS, CHUNK_SMEM, stream>>>(p);
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    }
+    scan_chunk_kernel<false><<<(unsigned)ctas, CHUNK_THREADS, CHUNK_SMEM, stream>>>(p);
+    return cudaGetLastError();
+}
+
+}  // namespace ssm
+}  // namespace gdn

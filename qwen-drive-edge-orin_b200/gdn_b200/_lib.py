@@ -43,10 +43,10 @@ SIGNATURES = {
     # include/gdn_ssm.h
     "causal_conv_prefill": (c_int, [c_void_p, c_int64] + [c_void_p] * 6 + [c_int] * 6 + [c_void_p]),
     "causal_conv_decode": (c_int, [c_void_p, c_int64] + [c_void_p] * 4 + [c_int] * 6 + [c_void_p]),
-    "selective_scan_workspace_size": (c_size_t, [c_int] * 7),
+    "selective_scan_scratch_size": (c_size_t, [c_int] * 7),
     "selective_scan_prefill": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64,
                                        c_void_p, c_int64, c_void_p, c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 6
-                               + [c_void_p, c_size_t, c_void_p]),
+                               + [c_void_p, c_size_t, c_void_p, c_size_t, c_void_p]),
     "selective_scan_decode": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64,
                                       c_void_p, c_int64, c_void_p, c_void_p, c_int] + [c_void_p] * 2 + [c_int] * 6
                               + [c_void_p]),

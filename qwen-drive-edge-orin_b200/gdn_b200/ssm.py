@@ -207,11 +207,12 @@ def _scan_prefill(x, dt, A, B, C, D, dt_bias, s0, dt_softplus, cu):
     y = torch.empty((b, T, H, P), dtype=torch.bfloat16, device=dev)
     sf = torch.empty((n, H, P, N), dtype=torch.float32, device=dev)
     lib = load_library()
-    nbytes = lib.selective_scan_workspace_size(n, T, int(cu is not None), H, P, G, N)
-    ws = _workspace(dev, nbytes)
+    nbytes = lib.selective_scan_scratch_size(n, T, int(cu is not None), H, P, G, N)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    ws = _workspace(dev, 256)  # the status word only
     _call(dev, "selective_scan_prefill", lib.selective_scan_prefill, _p(x), xs, _p(dt), dts, int(dt.dtype == torch.bfloat16),
           _p(A), _p(B), bs, _p(C), cs, _p(D), _p(dt_bias), int(bool(dt_softplus)), _p(s0), _p(y), _p(sf), _p(cu), n, T, H, P,
-          G, N, _p(ws), ws.numel())
+          G, N, _p(ws), ws.numel(), _p(scratch), nbytes)
     return [y, sf]
 
 

@@ -231,10 +231,11 @@ def test_scan_leaves_uncovered_rows():
     y = torch.full((1, T, H, P), 7.0, device=DEV, dtype=torch.bfloat16)
     sf = torch.empty(2, H, P, N, device=DEV)
     lib = gdn_b200.load_library()
-    ws = torch.zeros(lib.selective_scan_workspace_size(2, T, 1, H, P, G, N), dtype=torch.uint8, device=DEV)
+    ws = torch.zeros(256, dtype=torch.uint8, device=DEV)
+    scratch = torch.empty(lib.selective_scan_scratch_size(2, T, 1, H, P, G, N), dtype=torch.uint8, device=DEV)
     rc = lib.selective_scan_prefill(s["x"].data_ptr(), H * P, s["dt"].data_ptr(), H, 0, s["A"].data_ptr(), s["B"].data_ptr(), G * N,
                                     s["C"].data_ptr(), G * N, s["D"].data_ptr(), s["dt_bias"].data_ptr(), 1, None, y.data_ptr(),
-                                    sf.data_ptr(), cu.data_ptr(), 2, T, H, P, G, N, ws.data_ptr(), ws.numel(),
+                                    sf.data_ptr(), cu.data_ptr(), 2, T, H, P, G, N, ws.data_ptr(), 256, scratch.data_ptr(), scratch.numel(),
                                     torch.cuda.current_stream().cuda_stream)
     assert rc == 0
     assert (y[0, :5] == 7).all() and (y[0, 290:] == 7).all()

@@ -49,7 +49,7 @@ def test_empty_calls_are_no_ops():
 
 def _scan(**kw):
     a = dict(x=P, xs=128, dt=P, dts=2, dtb=0, A=P, B=P, bs=128, C=P, cs=128, D=None, bias=None, sp=1, s0=None, y=P, sf=P,
-             cu=None, N=1, T=4, H=2, P=64, G=1, NS=128, ws=P, wsb=1 << 30)
+             cu=None, N=1, T=4, H=2, P=64, G=1, NS=128, ws=P, wsb=256, scr=P, scrb=1 << 40)
     a.update(kw)
     return gdn_b200.load_library().selective_scan_prefill(*a.values(), None)
 
