@@ -9,14 +9,13 @@
 //
 // A CTA owns one segment of a sequence and two "slots" of a group: a slot is one head's tile of up to
 // 64 channels (a head of 128 is two slots). The two share the B and C tiles and G, and stand side by
-// side in the N = 128 columns of the inter-chunk and state products. Per chunk the tensor pipe runs
-// inter (C S^T), state (B^T X', three products, below), intra (M X) and the next chunk's G, in this
-// order, so that it has work while the warps form M, X' and the next state operand.
+// side in the N = 128 columns of the inter-chunk and state products.
 //   warps 0-7   slot 0 / slot 1: M (bf16) from G into TMEM, the A operand of M X; Y <- e^c Y; output tile
-//   warps 8-15  slot 0 / slot 1: X' pieces of 16 tokens into a ring; the state S^T (fp32, TMEM-resident):
+//   warps 8-15  slot 0 / slot 1: X' pieces of 32 tokens into a ring; the state S^T (fp32, TMEM-resident):
 //               its bf16 copy (operand of C S^T) and its decay
-//   warp 16     issues every MMA (one thread); warp 17 every TMA load; warp 18 the gates; warp 19 the
-//               TMA stores of the output tiles
+//   warp 16     issues the state products B^T X' (three per piece, below), warp 19 the others, per chunk
+//               inter (C S^T), intra (M X) and the next chunk's G
+//   warp 17     every TMA load and the TMA stores of the output tiles; warp 18 the gates
 //
 // Precision. G and all sums are fp32. M and the state operand of C S^T are rounded to bf16 once (y is
 // a bf16 output: together 1.0 of its own rounding error). The state itself is an fp32 output and carries
@@ -48,7 +47,7 @@ namespace ssm {
 
 constexpr int CH = 128;      // tokens per chunk
 constexpr int TILE = 64;     // channels per slot
-constexpr int PIECE = 16;    // tokens per piece of X'
+constexpr int PIECE = 32;    // tokens per piece of X'
 constexpr int PIECES = CH / PIECE;
 constexpr int WARPS = 20;
 constexpr int CHUNK_THREADS = 32 * WARPS;
@@ -56,21 +55,25 @@ constexpr int CHUNK_THREADS = 32 * WARPS;
 // ---- shared memory (bytes from a 1024-aligned base); bf16 tiles in the 128-byte swizzle TMA writes:
 // panels of 64 columns, rows of 128 bytes
 constexpr uint32_t PANEL = CH * 128;                 // 16 KB
-constexpr uint32_t OFF_B = 0;                        // 2 buffers x 2 panels [128 tokens][64 state]
-constexpr uint32_t OFF_C = OFF_B + 4 * PANEL;        // 2 panels
+constexpr uint32_t OFF_B = 0;                        // 2 panels [128 tokens][64 state]
+constexpr uint32_t OFF_C = OFF_B + 2 * PANEL;        // 2 panels (state pass: the second B buffer)
 constexpr uint32_t OFF_X = OFF_C + 2 * PANEL;        // 2 buffers x 2 slots [128 tokens][64 channels]; becomes y
 constexpr uint32_t OFF_S = OFF_X + 4 * PANEL;        // 2 slots [128 state][64 channels]
 constexpr uint32_t SUB = PIECE * 128;                // one slot's term of a piece
 constexpr uint32_t RING = 3 * 2 * SUB;               // a piece: 3 terms x 2 slots
-constexpr uint32_t OFF_R = OFF_S + 2 * PANEL;        // 2 pieces
-constexpr uint32_t OFF_GATE = OFF_R + 2 * RING;      // 2 buffers x 2 slots x Gates
+constexpr int RINGS = 2;                             // pieces in the ring
+constexpr uint32_t OFF_R = OFF_S + 2 * PANEL;
+constexpr uint32_t OFF_GATE = OFF_R + RINGS * RING;  // 2 buffers x 2 slots x Gates
 constexpr uint32_t GATE_BYTES = 4 * CH * 4;
 constexpr uint32_t OFF_MISC = OFF_GATE + 4 * GATE_BYTES;
 constexpr uint32_t MISC_SUMS = 0;                    // block sums [2 buffers][2 slots][4]
 constexpr uint32_t MISC_BAR = 64;
-constexpr uint32_t MISC_TMEM = 320;
-constexpr uint32_t MISC_SEG = 324;                   // sequence, segment in it, count, first, begin, length
-constexpr uint32_t MISC_BYTES = 384;
+constexpr uint32_t MISC_TMEM = 344;
+constexpr uint32_t MISC_SEG = 348;                   // the CTA's segment and slots:
+enum { SEG_SEQ, SEG_J, SEG_COUNT, SEG_FIRST, SEG_ROW, SEG_LEN, SEG_HEAD, SEG_TILE = SEG_HEAD + 2, SEG_SECOND = SEG_TILE + 2,
+       SEG_GROUP, SEG_PART, SEG_WORDS };
+constexpr uint32_t MISC_BYTES = 448;
+static_assert(MISC_SEG + 4 * SEG_WORDS <= MISC_BYTES, "segment words overflow");
 constexpr uint32_t CHUNK_SMEM = OFF_MISC + MISC_BYTES + 1024;
 static_assert(CHUNK_SMEM <= 232448, "exceeds the 227 KB per-block shared memory limit");
 
@@ -84,21 +87,25 @@ constexpr uint32_t TM_M = 128;   // M bf16 pairs, 64 columns per slot
 constexpr uint32_t TM_Y = 256;   // y fp32 [token][slot, channel]
 constexpr uint32_t TM_ST = 384;  // S^T fp32 [state][slot, channel]
 
-// Barriers. *F full, *E empty.
+// Barriers. *F full, *E empty. A phase is waited for by parity, so each is completed at most once more
+// before its last waiter has seen it: buffers that a thread reloads on it have a barrier each.
 enum {
-    B_XF = 0, B_XE = 2, B_BF = 4, B_BE = 6, B_CF = 8,
-    B_GF = 9,   // G in TMEM
-    B_ID = 10,  // inter product done (y's columns written, C tile free)
-    B_MR = 11,  // M written, y scaled, G read
-    B_YD = 12,  // intra product done
-    B_YF = 13,  // y's columns read
-    B_SC = 14,  // state operand written and state decayed
-    B_SD = 15,  // state product done
-    B_RF = 16, B_RE = 18,  // ring of X' pieces
-    B_PF = 20, B_PE = 22,  // gates
-    B_YS = 24,             // output tile written, per slot
-    B_DR = 26,             // every MMA done (exit)
-    NBARS = 27
+    B_XF = 0, B_XE = 2,  // (XE: state pass)
+    B_BF = 4,            // (two in the state pass)
+    B_CF = 6,
+    B_GF = 7,   // G in TMEM
+    B_ID = 8,   // inter product done (y's columns written, C tile free)
+    B_MR = 9,   // M written, y scaled, G read
+    B_YD = 10,  // intra product done
+    B_YF = 11,  // y's columns read
+    B_SC = 12,  // state operand written and state decayed
+    B_SD = 13,  // state product done
+    B_RF = 14, B_RE = 16,  // ring of X' pieces
+    B_PF = 18, B_PE = 20,  // gates
+    B_YS = 22,             // output tile written, per slot and buffer
+    B_DR = 26,             // every MMA of an issuing thread done (exit)
+    B_BE = 28,             // B buffers of the state pass
+    NBARS = 30
 };
 static_assert(MISC_BAR + 8 * NBARS <= MISC_TMEM, "barriers overlap the TMEM address word");
 
@@ -124,6 +131,41 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t sr
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
+// 32 TMEM columns as raw words, so that they can be changed and stored from the same registers.
+__device__ __forceinline__ void tmem_ld32u(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void scale32(uint32_t (&r)[32], uint64_t f) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+        float x0, x1;
+        f2_unpack(f2_mul(f2_pack(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), f), x0, x1);
+        r[j] = __float_as_uint(x0);
+        r[j + 1] = __float_as_uint(x1);
+    }
+}
+__device__ __forceinline__ uint32_t pack_bits(uint32_t a, uint32_t b) { return pack_bf16(__uint_as_float(a), __uint_as_float(b)); }
+// Address of a row of a 1024-aligned swizzled panel; its 16-byte chunk c is at that address ^ (c << 4).
+__device__ __forceinline__ uint32_t row_at(uint32_t panel, int row) { return panel + row * 128 + ((row & 7) << 4); }
+// Makes a value opaque here, so that what is derived from it is formed in place and not kept in
+// registers over a loop.
+__device__ __forceinline__ void keep_local(uint32_t& v) { asm volatile("" : "+r"(v)); }
+// One thread of a converged warp. Issuing threads are chosen by this and not by lane index: the compiler
+// then keeps an MMA's descriptors in uniform registers, without which an issue takes 80 cycles and more
+// (measured: 128 x 128 x 16 every 66 cycles against 89, 128 x 64 with A in TMEM 32 against 79).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
 __device__ __forceinline__ uint32_t top_halves(float a, float b) {  // bf16 pair of the leading halves
     return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
 }
@@ -143,8 +185,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
     auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
 
     // ---- this CTA's segment ----
-    const int unit = blockIdx.x % p.units, sid = blockIdx.x / p.units;
     if (warp == 0) {
+        const int unit = blockIdx.x % p.units, sid = blockIdx.x / p.units;
         int seq = sid, j = 0, first = sid, count = 1;
         if (p.seg_tokens > 0 && a.cu == nullptr) {
             count = max(1, (a.T + p.seg_tokens - 1) / p.seg_tokens);
@@ -184,21 +226,32 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
             if (seq < a.N) seq_range(a.cu, seq, a.T, b, e);
             // rows fit 31 bits (checked by the launcher)
             const int begin = (int)b + j * p.seg_tokens;
-            seg[0] = seq;
-            seg[1] = j;
-            seg[2] = count;
-            seg[3] = first;
-            seg[4] = begin;
-            seg[5] = (p.seg_tokens > 0) ? min(p.seg_tokens, (int)e - begin) : (int)(e - b);
+            seg[SEG_SEQ] = seq;
+            seg[SEG_J] = j;
+            seg[SEG_COUNT] = count;
+            seg[SEG_FIRST] = first;
+            seg[SEG_ROW] = begin;
+            seg[SEG_LEN] = (p.seg_tokens > 0) ? min(p.seg_tokens, (int)e - begin) : (int)(e - b);
+            // slots: head and channel tile; an odd one out runs its slot twice and stores it once
+            const int g = unit / p.pairs, r_heads = a.H / a.G, first_slot = 2 * (unit - g * p.pairs);
+            const bool second = first_slot + 1 < r_heads * p.ptiles;
+            for (int s = 0; s < 2; ++s) {
+                const int slot = first_slot + (second ? s : 0);
+                seg[SEG_HEAD + s] = g * r_heads + slot / p.ptiles;
+                seg[SEG_TILE + s] = slot % p.ptiles * TILE;
+            }
+            seg[SEG_SECOND] = second;
+            seg[SEG_GROUP] = g;
+            seg[SEG_PART] = blockIdx.x * 2;  // (segment, unit), slot 0
         }
     }
     if (tid == 32) {
         for (int i = 0; i < NBARS; ++i) {
             int n = 1;
-            if (i == B_MR || i == B_YF || i == B_SC || i == B_RF || i == B_RF + 1) n = 8;
+            if (i == B_MR || i == B_YF || i == B_SC || (i >= B_RF && i < B_RF + RINGS)) n = 8;
             if (i == B_PE || i == B_PE + 1) n = kState ? 8 : 16;
-            if (i == B_XE || i == B_XE + 1) n = kState ? 8 : 1;
-            if (i == B_YS || i == B_YS + 1) n = 4;
+            if (i == B_XE || i == B_XE + 1) n = 8;
+            if (i >= B_YS && i < B_YS + 4) n = 4;
             ptx::mbar_init(bar(i), n);
         }
         ptx::fence_mbar_init();
@@ -211,27 +264,33 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
     __syncthreads();
     ptx::tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + OFF_MISC + MISC_TMEM);
-    const int seq = seg[0], seg_j = seg[1], seg_count = seg[2], seg_first = seg[3];
-    const int row0 = seg[4], len = seg[5];
+    // What a role needs of these it reads where it needs it: kept in registers over the roles' loops they
+    // cost spills.
+    const int len = seg[SEG_LEN];
     // no such segment (the grid covers the most there can be); the state pass skips last segments
-    const bool idle = seq >= a.N || (kState && seg_j == seg_count - 1);
+    const bool idle = seg[SEG_SEQ] >= a.N || (kState && seg[SEG_J] == seg[SEG_COUNT] - 1);
     const int nc = idle ? 0 : (len + CH - 1) / CH;
-
-    // ---- slots: head and channel tile ----
-    const int g = unit / p.pairs, r_heads = a.H / a.G;
-    const int slot0 = 2 * (unit - g * p.pairs), nslots = r_heads * p.ptiles;
-    const bool second = slot0 + 1 < nslots;  // an odd one out runs its slot twice and stores it once
-    auto slot_head = [&](int s) { return g * r_heads + (slot0 + (second ? s : 0)) / p.ptiles; };
-    auto slot_tile = [&](int s) { return (slot0 + (second ? s : 0)) % p.ptiles; };
+    auto slot_head = [&](int s) { return (int)seg[SEG_HEAD + s]; };
+    auto slot_tile = [&](int s) { return (int)seg[SEG_TILE + s]; };
     const int npanel = a.NS > 64 ? 2 : 1;
 
-    // Waits are bounded; the vote keeps a warp together when one runs out.
-    auto wait = [&](int b, uint32_t parity) -> bool {
-        const bool ok = ptx::mbar_wait(bar(b), parity & 1u, WAIT_ITERS);
-        if (!ok) scan_wait_failed(p.status);
-        return ok;
+    // Waits are bounded. After one ran out a thread waits for nothing more: warps finish their loops on
+    // whatever is there (every access stays in its buffer), issuing threads stop.
+    bool dead = false;
+    auto wait = [&](int b, uint32_t parity) {
+        if (!dead && !ptx::mbar_wait(bar(b), parity & 1u, WAIT_ITERS)) {
+            dead = true;
+            scan_wait_failed(p.status);
+        }
     };
-    auto warp_wait = [&](int b, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(b, parity)); };
+    auto warp_wait = [&](int b, uint32_t parity) {
+        wait(b, parity);
+        __syncwarp();
+    };
+    // B tile of chunk k
+    auto b_off = [](int k) { return (kState && (k & 1)) ? OFF_C : OFF_B; };
+    auto b_bar = [](int k) { return kState ? B_BF + (k & 1) : B_BF; };
+    auto b_par = [](int k) { return kState ? (uint32_t)k >> 1 : (uint32_t)k; };
     auto warp_arrive = [&](int b) {
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar(b));
@@ -245,17 +304,18 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
         if constexpr (!kState) {
             const int s = warp >> 2, q = warp & 3, i = 32 * q + lane;
             const uint32_t tm_m = tl + TM_M + 64 * s, tm_y = tl + TM_Y + 64 * s;
-            const int h = slot_head(s), c0 = slot_tile(s) * TILE;
+            const int h = slot_head(s), c0 = slot_tile(s), row0 = seg[SEG_ROW];
             const float D = a.D ? a.D[h] : 0.f;
-            const bool stores = s == 0 || second;
+            const bool stores = s == 0 || seg[SEG_SECOND];
             if (nc > 0) {  // blocks right of the diagonal stay zero
                 const uint32_t zero[16] = {};
                 for (int b = q + 1; b < 4; ++b) ptx::tmem_st16(tm_m + 16 * b, zero);
             }
-            auto body = [&](int k) -> bool {
+            for (int k = 0; k < nc; ++k) {
                 const int buf = k & 1;
                 const uint32_t m = (uint32_t)k >> 1;
-                if (!warp_wait(B_PF + buf, m) || !warp_wait(B_GF, k)) return false;
+                warp_wait(B_PF + buf, m);
+                warp_wait(B_GF, k);
                 ptx::tc_fence_after();
                 const float* gt = gates(buf, s);
                 const float ci = gt[GT_C + i];
@@ -289,49 +349,46 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 {
                     float v[32];
                     ptx::tmem_ld32(tl + TM_G + 32 * q, v);
+                    const uint64_t cc = f2_pack(ci, ci);
                     uint32_t o[16];
                     ptx::tmem_wait_ld();
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
                         const float4 c4 = ld4(gt + GT_C + 32 * q + j), d4 = ld4(gt + GT_D + 32 * q + j);
+                        float e0, e1, e2, e3;
+                        f2_unpack(f2_sub(cc, f2_pack(c4.x, c4.y)), e0, e1);
+                        f2_unpack(f2_sub(cc, f2_pack(c4.z, c4.w)), e2, e3);
+                        f2_unpack(f2_mul(f2_mul(f2_pack(ex2f(e0), ex2f(e1)), f2_pack(d4.x, d4.y)), f2_pack(v[j], v[j + 1])), e0, e1);
+                        f2_unpack(f2_mul(f2_mul(f2_pack(ex2f(e2), ex2f(e3)), f2_pack(d4.z, d4.w)), f2_pack(v[j + 2], v[j + 3])), e2, e3);
                         // a select, not a product with zero: rows behind a sequence may hold anything
-                        const float x0 = j + 0 <= lane ? v[j + 0] * (ex2f(ci - c4.x) * d4.x) : 0.f;
-                        const float x1 = j + 1 <= lane ? v[j + 1] * (ex2f(ci - c4.y) * d4.y) : 0.f;
-                        const float x2 = j + 2 <= lane ? v[j + 2] * (ex2f(ci - c4.z) * d4.z) : 0.f;
-                        const float x3 = j + 3 <= lane ? v[j + 3] * (ex2f(ci - c4.w) * d4.w) : 0.f;
-                        o[j / 2] = pack_bf16(x0, x1);
-                        o[j / 2 + 1] = pack_bf16(x2, x3);
+                        o[j / 2] = pack_bf16(j + 0 <= lane ? e0 : 0.f, j + 1 <= lane ? e1 : 0.f);
+                        o[j / 2 + 1] = pack_bf16(j + 2 <= lane ? e2 : 0.f, j + 3 <= lane ? e3 : 0.f);
                     }
                     ptx::tmem_st16(tm_m + 16 * q, o);
                 }
                 // Y <- e^{c_i} (C S^T), so that M X accumulates onto it
                 const float e = ex2f(ci + before);
                 const uint64_t ee = f2_pack(e, e);
-                if (!warp_wait(B_ID, k)) return false;
+                warp_wait(B_ID, k);
                 ptx::tc_fence_after();
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    float v[32];
-                    uint32_t o[32];
-                    ptx::tmem_ld32(tm_y + 32 * hf, v);
+                    uint32_t v[32];
+                    tmem_ld32u(tm_y + 32 * hf, v);
                     ptx::tmem_wait_ld();
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        float x0, x1;
-                        f2_unpack(f2_mul(f2_pack(v[j], v[j + 1]), ee), x0, x1);
-                        o[j] = __float_as_uint(x0);
-                        o[j + 1] = __float_as_uint(x1);
-                    }
-                    ptx::tmem_st32(tm_y + 32 * hf, o);
+                    scale32(v, ee);
+                    ptx::tmem_st32(tm_y + 32 * hf, v);
                 }
                 ptx::tmem_wait_st();
                 ptx::tc_fence_before();
                 warp_arrive(B_MR);
                 if (lane == 0) ptx::mbar_arrive(bar(B_PE + buf));
                 // ---- output tile: y = Y + D x, in place of x ----
-                if (!warp_wait(B_XF + buf, m) || !warp_wait(B_YD, k)) return false;
+                warp_wait(B_XF + buf, m);
+                warp_wait(B_YD, k);
                 ptx::tc_fence_after();
-                const uint32_t xt = sb + OFF_X + (2 * buf + s) * PANEL;
+                uint32_t xt = row_at(sb + OFF_X + (2 * buf + s) * PANEL, i);
+                keep_local(xt);
                 const uint64_t dd = f2_pack(D, D);
                 const int valid = min(CH, len - CH * k);
                 const int64_t row = (int64_t)row0 + CH * k + i;
@@ -347,7 +404,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                     }
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        const uint32_t at = xt + sw_chunk(i, 4 * hf + c, CH);
+                        const uint32_t at = xt ^ ((4 * hf + c) << 4);
                         uint32_t u[4];
                         ld_shared_v4(at, u[0], u[1], u[2], u[3]);
 #pragma unroll
@@ -367,38 +424,33 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 }
                 if (valid == CH) {
                     ptx::fence_proxy_async_smem();
-                    warp_arrive(B_YS + s);
+                    warp_arrive(B_YS + 2 * s + buf);
                 }
-                return true;
-            };
-            for (int k = 0; k < nc; ++k)
-                if (!body(k)) break;
+            }
         }
     } else if (warp < 16) {
         // ================= X' and the state =================
         const int s = (warp >> 2) - 2, n = 32 * (warp & 3) + lane;
         const int t128 = tid & 127, pt = t128 >> 3, pc = t128 & 7;  // token and 16-byte chunk of a piece
         const uint32_t tm_s = tl + TM_ST + 64 * s;
-        const int h = slot_head(s), c0 = slot_tile(s) * TILE;
-        const bool stores = s == 0 || second;
-        const size_t sbase = (((size_t)(seq < a.N ? seq : 0) * a.H + h) * a.P + c0) * a.NS + n;
-        bool ok = !idle;
-        if (ok) {  // entry state: the initial state carried through the earlier segments
+        if (!idle) {  // entry state: the initial state carried through the earlier segments
+            const int c0 = slot_tile(s), seg_first = seg[SEG_FIRST], seg_j = seg[SEG_J], unit = blockIdx.x % p.units;
+            const size_t sbase = (((size_t)seg[SEG_SEQ] * a.H + slot_head(s)) * a.P + c0) * a.NS + n;
 #pragma unroll 1
-            for (int hf = 0; hf < 2; ++hf) {
-                float v[32];
+            for (int q4 = 0; q4 < 4; ++q4) {
+                float v[16];
 #pragma unroll
-                for (int c = 0; c < 32; ++c) {
-                    const int ch = 32 * hf + c;
+                for (int c = 0; c < 16; ++c) {
+                    const int ch = 16 * q4 + c;
                     v[c] = (!kState && a.s0 != nullptr && c0 + ch < a.P && n < a.NS) ? a.s0[sbase + (size_t)ch * a.NS] : 0.f;
                 }
                 if constexpr (!kState) {
                     for (int e = seg_first; e < seg_first + seg_j; ++e) {
                         const size_t at = ((size_t)e * p.units + unit) * 2 + s;
                         const float decay = ex2f(p.part_log[at]);
-                        const float4* src = p.part + (at * (TILE / 4) + 8 * hf) * CH + n;
+                        const float4* src = p.part + (at * (TILE / 4) + 4 * q4) * CH + n;
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) {
+                        for (int c = 0; c < 4; ++c) {
                             const float4 f = src[c * CH];
                             v[4 * c] = fmaf(decay, v[4 * c], f.x);
                             v[4 * c + 1] = fmaf(decay, v[4 * c + 1], f.y);
@@ -407,130 +459,134 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                         }
                     }
                 }
-                uint32_t o[32];
+                uint32_t o[16];
 #pragma unroll
-                for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(v[c]);
-                ptx::tmem_st32(tm_s + 32 * hf, o);
+                for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(v[c]);
+                ptx::tmem_st16(tm_s + 16 * q4, o);
             }
             ptx::tmem_wait_st();
         }
         float log_decay = 0.f;
-        // piece i of chunk k: 16 tokens x 64 channels of X' = w x as three bf16 terms
-        auto piece = [&](int k, int i, int valid, const float* gt) -> bool {
-            const uint32_t use = (uint32_t)(PIECES * k + i) >> 1, slot = (uint32_t)i & 1u;
-            if (use > 0 && !warp_wait(B_RE + slot, use - 1)) return false;
-            const int t = PIECE * i + pt;
-            const float w = gt[GT_W + t];
-            const uint64_t ww = f2_pack(w, w);
-            uint32_t u[4], hi[4], mid[4], lo[4];
-            ld_shared_v4(sb + OFF_X + (2 * (k & 1) + s) * PANEL + sw_chunk(t, pc, CH), u[0], u[1], u[2], u[3]);
+        // piece i of chunk k: 32 tokens x 64 channels of X' = w x as three bf16 terms, tokens pt and pt + 16
+        // in this thread (16 token rows further on the swizzle is the same, so offsets advance by 2 KB)
+        const uint32_t x_at = sb + OFF_X + s * PANEL + sw_chunk(pt, pc, CH), r_at = sb + OFF_R + s * SUB + sw_chunk(pt, pc, PIECE);
+        auto piece = [&](int k, int i, const float* gt) {
+            const uint32_t use = (uint32_t)(PIECES * k + i) / RINGS, slot = (uint32_t)i % RINGS;
+            uint32_t u[8];
+            const uint32_t from = x_at + (uint32_t)(k & 1) * 2 * PANEL + (uint32_t)i * (PIECE * 128), to = r_at + slot * RING;
+            ld_shared_v4(from, u[0], u[1], u[2], u[3]);
+            ld_shared_v4(from + 2048, u[4], u[5], u[6], u[7]);
+            const float w0 = gt[GT_W + PIECE * i + pt], w1 = gt[GT_W + PIECE * i + pt + 16];
+            if (use > 0) warp_wait(B_RE + slot, use - 1);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t x = t < valid ? u[e] : 0u;
-                const uint64_t v = f2_mul(f2_pack(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u)), ww);
-                float v0, v1, r0, r1, l0, l1;
-                f2_unpack(v, v0, v1);
-                hi[e] = top_halves(v0, v1);
-                const uint64_t r = f2_sub(v, f2_pack(head(v0), head(v1)));
-                f2_unpack(r, r0, r1);
-                mid[e] = top_halves(r0, r1);
-                f2_unpack(f2_sub(r, f2_pack(head(r0), head(r1))), l0, l1);
-                lo[e] = top_halves(l0, l1);
+            for (int t = 0; t < 2; ++t) {
+                const uint64_t ww = t ? f2_pack(w1, w1) : f2_pack(w0, w0);
+                uint32_t hi[4], mid[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t x = u[4 * t + e];
+                    const uint64_t v = f2_mul(f2_pack(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u)), ww);
+                    float v0, v1, r0, r1, l0, l1;
+                    f2_unpack(v, v0, v1);
+                    hi[e] = top_halves(v0, v1);
+                    const uint64_t r = f2_sub(v, f2_pack(head(v0), head(v1)));
+                    f2_unpack(r, r0, r1);
+                    mid[e] = top_halves(r0, r1);
+                    f2_unpack(f2_sub(r, f2_pack(head(r0), head(r1))), l0, l1);
+                    lo[e] = top_halves(l0, l1);
+                }
+                st_shared_v4(to + 2048 * t, hi[0], hi[1], hi[2], hi[3]);
+                st_shared_v4(to + 2 * SUB + 2048 * t, mid[0], mid[1], mid[2], mid[3]);
+                st_shared_v4(to + 4 * SUB + 2048 * t, lo[0], lo[1], lo[2], lo[3]);
             }
-            const uint32_t at = sb + OFF_R + slot * RING + s * SUB + sw_chunk(pt, pc, PIECE);
-            st_shared_v4(at, hi[0], hi[1], hi[2], hi[3]);
-            st_shared_v4(at + 2 * SUB, mid[0], mid[1], mid[2], mid[3]);
-            st_shared_v4(at + 4 * SUB, lo[0], lo[1], lo[2], lo[3]);
             ptx::fence_proxy_async_smem();
             warp_arrive(B_RF + slot);
-            return true;
         };
-        auto body = [&](int k) -> bool {
+        for (int k = 0; k < nc; ++k) {
             const int buf = k & 1;
             const uint32_t m = (uint32_t)k >> 1;
             const int valid = min(CH, len - CH * k);
-            if (!warp_wait(B_PF + buf, m) || !warp_wait(B_XF + buf, m)) return false;
+            warp_wait(B_PF + buf, m);
+            warp_wait(B_XF + buf, m);
             if (valid < CH) {
                 // the rows behind the sequence belong to others and may hold anything: zeros in X and B,
                 // whose products would otherwise reach valid rows as 0 x NaN
-                if (!warp_wait(B_BF + buf, m)) return false;
+                warp_wait(b_bar(k), b_par(k));
                 for (int e = t128; e < (CH - valid) * 8; e += 128) {
                     const uint32_t off = sw_chunk(valid + (e >> 3), e & 7, CH);
                     st_shared_v4(sb + OFF_X + (2 * buf + s) * PANEL + off, 0, 0, 0, 0);
-                    if (s < npanel) st_shared_v4(sb + OFF_B + (2 * buf + s) * PANEL + off, 0, 0, 0, 0);
+                    if (s < npanel) st_shared_v4(sb + b_off(k) + s * PANEL + off, 0, 0, 0, 0);
                 }
                 ptx::fence_proxy_async_smem();
+                ptx::named_sync(1 + s, 128);
             }
             const float* gt = gates(buf, s);
-            if (!piece(k, 0, valid, gt) || !piece(k, 1, valid, gt)) return false;
+#pragma unroll 1
+            for (int i = 0; i < RINGS; ++i) piece(k, i, gt);
             // the state: bf16 copy as the operand of C S^T, and its decay over this chunk
-            if (k > 0 && !warp_wait(B_SD, k - 1)) return false;
+            if (k > 0) warp_wait(B_SD, k - 1);
+            if (!kState && k > 0) warp_wait(B_ID, k - 1);  // the last operand has been read
             ptx::tc_fence_after();
             const float* R = sums + (2 * buf + s) * 4;
             const float total = (R[0] + R[1]) + (R[2] + R[3]);
             log_decay += total;
             const float decay = ex2f(total);
             const uint64_t dd = f2_pack(decay, decay);
-#pragma unroll
+#pragma unroll 1
             for (int hf = 0; hf < 2; ++hf) {
-                float v[32];
-                uint32_t o[32];
-                ptx::tmem_ld32(tm_s + 32 * hf, v);
+                uint32_t v[32];
+                tmem_ld32u(tm_s + 32 * hf, v);
                 ptx::tmem_wait_ld();
                 if constexpr (!kState) {
+                    uint32_t at = row_at(sb + OFF_S + s * PANEL, n);
+                    keep_local(at);
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
-                        st_shared_v4(sb + OFF_S + s * PANEL + sw_chunk(n, 4 * hf + c, CH), pack_bf16(v[8 * c], v[8 * c + 1]),
-                                     pack_bf16(v[8 * c + 2], v[8 * c + 3]), pack_bf16(v[8 * c + 4], v[8 * c + 5]),
-                                     pack_bf16(v[8 * c + 6], v[8 * c + 7]));
+                        st_shared_v4(at ^ ((4 * hf + c) << 4), pack_bits(v[8 * c], v[8 * c + 1]),
+                                     pack_bits(v[8 * c + 2], v[8 * c + 3]), pack_bits(v[8 * c + 4], v[8 * c + 5]),
+                                     pack_bits(v[8 * c + 6], v[8 * c + 7]));
                 }
-#pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                    float x0, x1;
-                    f2_unpack(f2_mul(f2_pack(v[j], v[j + 1]), dd), x0, x1);
-                    o[j] = __float_as_uint(x0);
-                    o[j + 1] = __float_as_uint(x1);
-                }
-                ptx::tmem_st32(tm_s + 32 * hf, o);
+                scale32(v, dd);
+                ptx::tmem_st32(tm_s + 32 * hf, v);
             }
             ptx::tmem_wait_st();
             ptx::fence_proxy_async_smem();
             ptx::tc_fence_before();
             warp_arrive(B_SC);
 #pragma unroll 1
-            for (int i = 2; i < PIECES; ++i)
-                if (!piece(k, i, valid, gt)) return false;
+            for (int i = RINGS; i < PIECES; ++i) piece(k, i, gt);
             warp_arrive(B_PE + buf);
             if (kState) warp_arrive(B_XE + buf);
-            return true;
-        };
-        for (int k = 0; ok && k < nc; ++k) ok = body(k);
-        if (ok && nc > 0) {
-            ok = warp_wait(B_SD, nc - 1);
+        }
+        if (nc > 0) {
+            warp_wait(B_SD, nc - 1);
             ptx::tc_fence_after();
         }
-        if (ok && (kState || seg_j == seg_count - 1)) {
-            const size_t at = ((size_t)sid * p.units + unit) * 2 + s;
+        if (!idle && (kState || seg[SEG_J] == seg[SEG_COUNT] - 1)) {
+            const int c0 = slot_tile(s);
+            const bool stores = s == 0 || seg[SEG_SECOND];
+            const size_t sbase = (((size_t)seg[SEG_SEQ] * a.H + slot_head(s)) * a.P + c0) * a.NS + n;
+            const size_t at = (size_t)seg[SEG_PART] + s;
             if (kState && n == 0) p.part_log[at] = log_decay;
 #pragma unroll 1
-            for (int hf = 0; hf < 2; ++hf) {
-                float v[32];
-                ptx::tmem_ld32(tm_s + 32 * hf, v);
+            for (int q4 = 0; q4 < 4; ++q4) {
+                float v[16];
+                ptx::tmem_ld16(tm_s + 16 * q4, v);
                 ptx::tmem_wait_ld();
                 if (kState) {
 #pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        p.part[(at * (TILE / 4) + 8 * hf + c) * CH + n] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+                    for (int c = 0; c < 4; ++c)
+                        p.part[(at * (TILE / 4) + 4 * q4 + c) * CH + n] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
                 } else if (stores && n < a.NS) {
 #pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (c0 + 32 * hf + c < a.P) a.sf[sbase + (size_t)(32 * hf + c) * a.NS] = v[c];
+                    for (int c = 0; c < 16; ++c)
+                        if (c0 + 16 * q4 + c < a.P) a.sf[sbase + (size_t)(16 * q4 + c) * a.NS] = v[c];
                 }
             }
         }
-    } else if (warp == 16) {
-        // ================= MMA issue (one thread) =================
-        if (lane == 0) {
+    } else if (warp == 16 || warp == 19) {
+        // ================= MMA issue (one thread of each warp) =================
+        if (elect_one()) {
             constexpr uint32_t ID_G = ptx::idesc_bf16(128, 128, 0, 0, 0);      // C B^T
             constexpr uint32_t ID_INTER = ptx::idesc_bf16(128, 128, 0, 1, 0);  // C S^T       (B MN-major)
             constexpr uint32_t ID_STATE = ptx::idesc_bf16(128, 128, 1, 1, 0);  // B^T X'      (both MN-major)
@@ -538,122 +594,166 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
             const uint32_t d16 = ptx::sw128_desc_lo(sb, 16), dpanel = ptx::sw128_desc_lo(sb, PANEL), dsub = ptx::sw128_desc_lo(sb, SUB);
             auto desc = [](uint32_t base, uint32_t off) { return ptx::desc_pair(base + (off >> 4), ptx::sw128_desc_hi(1024)); };
             auto kmajor = [](int st) { return (uint32_t)(st >> 2) * PANEL + (uint32_t)(st & 3) * 32u; };
-            const int ks = (a.NS + 15) / 16;  // K steps over the state dimension
-            auto issue_g = [&](int k) -> bool {
-                if (!wait(B_BF + (k & 1), (uint32_t)k >> 1) || !wait(B_CF, k)) return false;
-                ptx::tc_fence_after();
-                for (int st = 0; st < ks; ++st)
-                    ptx::mma_bf16(tmem + TM_G, desc(d16, OFF_C + kmajor(st)), desc(d16, OFF_B + (k & 1) * 2 * PANEL + kmajor(st)), ID_G, st > 0);
-                ptx::mma_commit(bar(B_GF));
-                return true;
-            };
-            auto body = [&](int k) -> bool {
-                const int buf = k & 1;
-                if (kState) {
-                    if (!wait(B_BF + buf, (uint32_t)k >> 1)) return false;
+            if (warp == 16) {
+                for (int k = 0; k < nc; ++k) {
+                    wait(b_bar(k), b_par(k));
+                    wait(B_SC, k);
+                    for (int i = 0; i < PIECES && !dead; ++i) {
+                        const uint32_t use = (uint32_t)(PIECES * k + i) / RINGS, slot = (uint32_t)i % RINGS;
+                        wait(B_RF + slot, use);
+                        if (dead) break;
+                        ptx::tc_fence_after();
+#pragma unroll
+                        for (int st = 0; st < PIECE / 16; ++st)
+#pragma unroll
+                            for (int term = 0; term < 3; ++term)
+                                ptx::mma_bf16(tmem + TM_ST, desc(dpanel, b_off(k) + i * (PIECE * 128u) + st * 2048u),
+                                              desc(dsub, OFF_R + slot * RING + term * 2 * SUB + st * 2048u), ID_STATE, 1);
+                        ptx::mma_commit(bar(B_RE + slot));
+                    }
+                    if (dead) break;
+                    ptx::mma_commit(bar(B_SD));
+                    if (kState) ptx::mma_commit(bar(B_BE + (k & 1)));
                 }
-                if (!wait(B_SC, k)) return false;
-                if constexpr (!kState) {
-                    if (k > 0 && !wait(B_YF, k - 1)) return false;
+            } else if (!kState) {
+                const int ks = (a.NS + 15) / 16;  // K steps over the state dimension
+                auto issue_g = [&](int k) {
+                    wait(B_BF, k);
+                    wait(B_CF, k);
+                    if (dead) return;
+                    ptx::tc_fence_after();
+                    for (int st = 0; st < ks; ++st)
+                        ptx::mma_bf16(tmem + TM_G, desc(d16, OFF_C + kmajor(st)), desc(d16, OFF_B + kmajor(st)), ID_G, st > 0);
+                    ptx::mma_commit(bar(B_GF));
+                };
+                if (nc > 0) issue_g(0);
+                for (int k = 0; k < nc; ++k) {
+                    wait(B_SC, k);
+                    if (k > 0) wait(B_YF, k - 1);
+                    if (dead) break;
                     ptx::tc_fence_after();
                     for (int st = 0; st < ks; ++st)
                         ptx::mma_bf16(tmem + TM_Y, desc(d16, OFF_C + kmajor(st)), desc(dpanel, OFF_S + st * 2048u), ID_INTER, st > 0);
                     ptx::mma_commit(bar(B_ID));
-                }
-                ptx::tc_fence_after();
-                for (int i = 0; i < PIECES; ++i) {
-                    const uint32_t use = (uint32_t)(PIECES * k + i) >> 1, slot = (uint32_t)i & 1u;
-                    if (!wait(B_RF + slot, use)) return false;
-                    ptx::tc_fence_after();
-                    const uint64_t ad = desc(dpanel, OFF_B + buf * 2 * PANEL + i * 2048u);
-#pragma unroll
-                    for (int term = 0; term < 3; ++term)
-                        ptx::mma_bf16(tmem + TM_ST, ad, desc(dsub, OFF_R + slot * RING + term * 2 * SUB), ID_STATE, 1);
-                    ptx::mma_commit(bar(B_RE + slot));
-                }
-                ptx::mma_commit(bar(B_SD));
-                ptx::mma_commit(bar(B_BE + buf));
-                if constexpr (!kState) {
-                    if (!wait(B_MR, k)) return false;
+                    wait(B_MR, k);
+                    if (len - CH * k < CH)  // rows of X zeroed behind the sequence's end (before the first piece)
+                        wait(B_RF + RINGS - 1, (uint32_t)(PIECES * k + PIECES - 1) / RINGS);
+                    if (dead) break;
                     ptx::tc_fence_after();
 #pragma unroll
                     for (int s = 0; s < 2; ++s)
 #pragma unroll
-                        for (int st = 0; st < PIECES; ++st)
+                        for (int st = 0; st < CH / 16; ++st)
                             ptx::mma_bf16_ts(tmem + TM_Y + 64 * s, tmem + TM_M + 64 * s + 8 * st,
-                                             desc(d16, OFF_X + (2 * buf + s) * PANEL + st * 2048u), ID_INTRA, 1);
+                                             desc(d16, OFF_X + (2 * (k & 1) + s) * PANEL + st * 2048u), ID_INTRA, 1);
                     ptx::mma_commit(bar(B_YD));
-                    if (k + 1 < nc && !issue_g(k + 1)) return false;
+                    if (k + 1 < nc) issue_g(k + 1);
+                    if (dead) break;
                 }
-                return true;
-            };
-            bool ok = true;
-            if (!kState && nc > 0) ok = issue_g(0);
-            for (int k = 0; ok && k < nc; ++k) ok = body(k);
-            ptx::mma_commit(bar(B_DR));  // nothing in flight when the CTA leaves
-            wait(B_DR, 0);
+            }
+            // nothing in flight when the CTA leaves
+            const bool failed = dead;
+            dead = false;
+            ptx::mma_commit(bar(B_DR + (warp == 19)));
+            wait(B_DR + (warp == 19), 0);
+            dead |= failed;
         }
         __syncwarp();
     } else if (warp == 17) {
-        // ================= TMA loads (one thread) =================
-        if (lane == 0) {
+        // ================= TMA (one thread) =================
+        if (elect_one()) {
             ptx::prefetch_tensormap(&p.tm_x);
             ptx::prefetch_tensormap(&p.tm_b);
             if (!kState) ptx::prefetch_tensormap(&p.tm_c);
-            const int h0 = slot_head(0), h1 = slot_head(1), t0 = slot_tile(0) * TILE, t1 = slot_tile(1) * TILE;
+            const int h0 = slot_head(0), h1 = slot_head(1), t0 = slot_tile(0), t1 = slot_tile(1), row0 = seg[SEG_ROW], g = seg[SEG_GROUP];
+            const bool second = seg[SEG_SECOND];
             int nb = 0, nx = 0, ncl = 0;  // loads issued
-            auto body = [&](int k) -> bool {
-                const int buf = k & 1, row = row0 + CH * k;
-                const uint32_t m = (uint32_t)k >> 1;
-                if (m > 0 && !wait(B_BE + buf, m - 1)) return false;
+            auto load_b = [&](int k) {
+                if (dead || k >= nc) return;
                 ++nb;
-                ptx::mbar_arrive_expect_tx(bar(B_BF + buf), npanel * PANEL);
+                ptx::mbar_arrive_expect_tx(bar(b_bar(k)), npanel * PANEL);
                 for (int c = 0; c < npanel; ++c)
-                    ptx::tma_load_4d(sb + OFF_B + (2 * buf + c) * PANEL, &p.tm_b, bar(B_BF + buf), 64 * c, g, row, 0);
-                if (!kState && k == 0) {
-                    ++ncl;
-                    ptx::mbar_arrive_expect_tx(bar(B_CF), npanel * PANEL);
-                    for (int c = 0; c < npanel; ++c) ptx::tma_load_4d(sb + OFF_C + c * PANEL, &p.tm_c, bar(B_CF), 64 * c, g, row, 0);
-                }
-                if (m > 0 && !wait(B_XE + buf, m - 1)) return false;
-                ++nx;
-                ptx::mbar_arrive_expect_tx(bar(B_XF + buf), 2 * PANEL);
-                ptx::tma_load_4d(sb + OFF_X + 2 * buf * PANEL, &p.tm_x, bar(B_XF + buf), t0, h0, row, 0);
-                ptx::tma_load_4d(sb + OFF_X + (2 * buf + 1) * PANEL, &p.tm_x, bar(B_XF + buf), t1, h1, row, 0);
-                if (!kState && k > 0) {
-                    if (!wait(B_ID, k - 1)) return false;
-                    ++ncl;
-                    ptx::mbar_arrive_expect_tx(bar(B_CF), npanel * PANEL);
-                    for (int c = 0; c < npanel; ++c) ptx::tma_load_4d(sb + OFF_C + c * PANEL, &p.tm_c, bar(B_CF), 64 * c, g, row, 0);
-                }
-                return true;
+                    ptx::tma_load_4d(sb + b_off(k) + c * PANEL, &p.tm_b, bar(b_bar(k)), 64 * c, g, row0 + CH * k, 0);
             };
-            for (int k = 0; k < nc; ++k)
-                if (!body(k)) break;
-            // no load in flight when the CTA leaves
+            auto load_c = [&](int k) {
+                if (dead || k >= nc) return;
+                ++ncl;
+                ptx::mbar_arrive_expect_tx(bar(B_CF), npanel * PANEL);
+                for (int c = 0; c < npanel; ++c) ptx::tma_load_4d(sb + OFF_C + c * PANEL, &p.tm_c, bar(B_CF), 64 * c, g, row0 + CH * k, 0);
+            };
+            auto load_x = [&](int k) {
+                if (dead || k >= nc) return;
+                ++nx;
+                const int buf = k & 1;
+                ptx::mbar_arrive_expect_tx(bar(B_XF + buf), 2 * PANEL);
+                ptx::tma_load_4d(sb + OFF_X + 2 * buf * PANEL, &p.tm_x, bar(B_XF + buf), t0, h0, row0 + CH * k, 0);
+                ptx::tma_load_4d(sb + OFF_X + (2 * buf + 1) * PANEL, &p.tm_x, bar(B_XF + buf), t1, h1, row0 + CH * k, 0);
+            };
+            load_x(0);
+            load_b(0);
+            if (!kState) load_c(0);
+            if (kState) load_b(1);
+            load_x(1);
+            for (int k = 0; k < nc && !dead; ++k) {
+                if constexpr (kState) {
+                    wait(B_XE + (k & 1), (uint32_t)k >> 1);
+                    load_x(k + 2);
+                    wait(B_BE + (k & 1), (uint32_t)k >> 1);
+                    load_b(k + 2);
+                } else {
+                    if (k + 1 < nc) {  // the next tiles on their way to L2 while their buffers are in use
+                        for (int c = 0; c < npanel; ++c) {
+                            ptx::tma_prefetch_4d(&p.tm_b, 64 * c, g, row0 + CH * (k + 1), 0);
+                            ptx::tma_prefetch_4d(&p.tm_c, 64 * c, g, row0 + CH * (k + 1), 0);
+                        }
+                    }
+                    wait(B_ID, k);
+                    load_c(k + 1);
+                    wait(B_SD, k);
+                    wait(B_GF, k);
+                    load_b(k + 1);
+                    if (len - CH * k >= CH) {  // a full tile: out by TMA (the warps store a partial one themselves)
+                        const int buf = k & 1, row = row0 + CH * k;
+                        wait(B_YS + buf, (uint32_t)k >> 1);
+                        if (!dead) tma_store_4d(&p.tm_y, sb + OFF_X + 2 * buf * PANEL, t0, h0, row, 0);
+                        wait(B_YS + 2 + buf, (uint32_t)k >> 1);
+                        if (!dead && second) tma_store_4d(&p.tm_y, sb + OFF_X + (2 * buf + 1) * PANEL, t1, h1, row, 0);
+                        ptx::bulk_wait_read_all();
+                        load_x(k + 2);
+                    }
+                }
+            }
+            // nothing in flight when the CTA leaves
+            const bool failed = dead;
+            dead = false;
             for (int buf = 0; buf < 2; ++buf) {
-                if (nb > buf) wait(B_BF + buf, (uint32_t)(nb - 1 - buf) >> 1);
+                if (kState && nb > buf) wait(B_BF + buf, (uint32_t)(nb - 1 - buf) >> 1);
                 if (nx > buf) wait(B_XF + buf, (uint32_t)(nx - 1 - buf) >> 1);
             }
+            if (!kState && nb > 0) wait(B_BF, (uint32_t)(nb - 1));
             if (ncl > 0) wait(B_CF, (uint32_t)(ncl - 1));
+            ptx::bulk_wait_all();
+            dead |= failed;
         }
         __syncwarp();
     } else if (warp == 18) {
         // ================= gates of both slots =================
         float A2[2], bias[2], next[2][4];
+        const int row0 = seg[SEG_ROW], hd[2] = {slot_head(0), slot_head(1)};
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            A2[s] = a.A[slot_head(s)] * LOG2E;
-            bias[s] = a.dt_bias ? a.dt_bias[slot_head(s)] : 0.f;
+            A2[s] = a.A[hd[s]] * LOG2E;
+            bias[s] = a.dt_bias ? a.dt_bias[hd[s]] : 0.f;
         }
         auto load = [&](int k) {  // clamped to the segment's rows
             const int last = len - 1 - CH * k;
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) next[s][i] = scan_dt(a, (int64_t)row0 + CH * k + min(4 * lane + i, last), slot_head(s));
+                for (int i = 0; i < 4; ++i) next[s][i] = scan_dt(a, (int64_t)row0 + CH * k + min(4 * lane + i, last), hd[s]);
         };
-        auto body = [&](int k) -> bool {
+        if (nc > 0) load(0);
+        for (int k = 0; k < nc; ++k) {
             const int buf = k & 1, valid = len - CH * k;
             float d[2][4];
 #pragma unroll
@@ -665,7 +765,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                     d[s][i] = 4 * lane + i < valid ? v : 0.f;
                 }
             if (k + 1 < nc) load(k + 1);
-            if (k >= 2 && !warp_wait(B_PE + buf, ((uint32_t)k >> 1) - 1)) return false;
+            if (k >= 2) warp_wait(B_PE + buf, ((uint32_t)k >> 1) - 1);
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 // log2 decays; the clamp keeps sums of 128 finite, and 2^-1e30 is zero as well
@@ -705,27 +805,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 if (lane == 0) *reinterpret_cast<float4*>(sums + (2 * buf + s) * 4) = make_float4(R[0], R[1], R[2], R[3]);
             }
             warp_arrive(B_PF + buf);
-            return true;
-        };
-        if (nc > 0) load(0);
-        for (int k = 0; k < nc; ++k)
-            if (!body(k)) break;
-    } else {
-        // ================= TMA stores of full output tiles (one thread) =================
-        if (!kState && lane == 0) {
-            const int h0 = slot_head(0), h1 = slot_head(1), t0 = slot_tile(0) * TILE, t1 = slot_tile(1) * TILE;
-            for (int k = 0; k < nc && len - CH * k >= CH; ++k) {
-                const int buf = k & 1, row = row0 + CH * k;
-                if (!wait(B_YS, k)) break;
-                tma_store_4d(&p.tm_y, sb + OFF_X + 2 * buf * PANEL, t0, h0, row, 0);
-                if (!wait(B_YS + 1, k)) break;
-                if (second) tma_store_4d(&p.tm_y, sb + OFF_X + (2 * buf + 1) * PANEL, t1, h1, row, 0);
-                ptx::bulk_wait_read_all();
-                ptx::mbar_arrive(bar(B_XE + buf));
-            }
-            ptx::bulk_wait_all();
         }
-        __syncwarp();
     }
     ptx::tc_fence_before();
     __syncthreads();
