@@ -10,9 +10,10 @@
 // A CTA owns one segment of a sequence and two "slots" of a group: a slot is one head's tile of up to
 // 64 channels (a head of 128 is two slots). The two share the B and C tiles and G, and stand side by
 // side in the N = 128 columns of the inter-chunk and state products.
-//   warps 0-7   slot 0 / slot 1: M (bf16) from G into TMEM, the A operand of M X; Y <- e^c Y; output tile
-//   warps 8-15  slot 0 / slot 1: X' pieces of 32 tokens into a ring; the state S^T (fp32, TMEM-resident):
-//               its bf16 copy (operand of C S^T) and its decay
+//   warps 0-7   slot 0 / slot 1: M (bf16) from G into TMEM, the A operand of M X; Y <- e^c Y; the first
+//               half of X', in pieces of 32 tokens into a ring
+//   warps 8-15  slot 0 / slot 1: the state S^T (fp32, TMEM-resident): its bf16 copy (operand of C S^T)
+//               and its decay; the output tile; the second half of X'
 //   warp 16     issues the state products B^T X' (three per piece, below), warp 19 the others, per chunk
 //               inter (C S^T), intra (M X) and the next chunk's G
 //   warp 17     every TMA load and the TMA stores of the output tiles; warp 18 the gates
@@ -87,8 +88,10 @@ constexpr uint32_t TM_M = 128;   // M bf16 pairs, 64 columns per slot
 constexpr uint32_t TM_Y = 256;   // y fp32 [token][slot, channel]
 constexpr uint32_t TM_ST = 384;  // S^T fp32 [state][slot, channel]
 
-// Barriers. *F full, *E empty. A phase is waited for by parity, so each is completed at most once more
-// before its last waiter has seen it: buffers that a thread reloads on it have a barrier each.
+// Barriers. *F full, *E empty. A phase is waited for by its parity, so a waiter may neither skip a
+// phase nor let two complete before it looks: every waiter below waits for each phase of its barrier
+// in turn (or behind a wait that implies the phase before), and what it does next is needed for the
+// phase after.
 enum {
     B_XF = 0, B_XE = 2,  // (XE: state pass)
     B_BF = 4,            // (two in the state pass)
@@ -100,13 +103,15 @@ enum {
     B_YF = 11,  // y's columns read
     B_SC = 12,  // state operand written and state decayed
     B_SD = 13,  // state product done
-    B_RF = 14, B_RE = 16,  // ring of X' pieces
-    B_PF = 18, B_PE = 20,  // gates
-    B_YS = 22,             // output tile written, per slot and buffer
-    B_DR = 26,             // every MMA of an issuing thread done (exit)
-    B_BE = 28,             // B buffers of the state pass
-    NBARS = 30
+    B_RF = 14,             // ring of X' pieces: full
+    B_RE = 16,             // empty, per half of the chunk that has been read (each half has its writers)
+    B_PF = 20, B_PE = 22,  // gates
+    B_YS = 24,             // output tile written, per slot and buffer
+    B_DR = 28,             // every MMA of an issuing thread done (exit)
+    B_BE = 30,             // B buffers of the state pass
+    NBARS = 32
 };
+static_assert(PIECES == 2 * RINGS, "a ring holds half a chunk");
 static_assert(MISC_BAR + 8 * NBARS <= MISC_TMEM, "barriers overlap the TMEM address word");
 
 struct ChunkParams {
@@ -152,12 +157,41 @@ __device__ __forceinline__ void scale32(uint32_t (&r)[32], uint64_t f) {
         r[j + 1] = __float_as_uint(x1);
     }
 }
+// 16 columns from the first half of a 32-word buffer.
+__device__ __forceinline__ void store16(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
 __device__ __forceinline__ uint32_t pack_bits(uint32_t a, uint32_t b) { return pack_bf16(__uint_as_float(a), __uint_as_float(b)); }
 // Address of a row of a 1024-aligned swizzled panel; its 16-byte chunk c is at that address ^ (c << 4).
 __device__ __forceinline__ uint32_t row_at(uint32_t panel, int row) { return panel + row * 128 + ((row & 7) << 4); }
 // Makes a value opaque here, so that what is derived from it is formed in place and not kept in
 // registers over a loop.
 __device__ __forceinline__ void keep_local(uint32_t& v) { asm volatile("" : "+r"(v)); }
+// v[j] <- bf16 pairs of v[j] h[j] f where bit j of `keep` is set, else 0 (a select, not a product with
+// zero: rows behind a sequence may hold anything).
+__device__ __forceinline__ void form_m(uint32_t (&v)[32], const float* h, float f, uint32_t keep) {
+    const uint64_t ff = f2_pack(f, f);
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+        const float4 h4 = ld4(h + j);
+        float x0, x1, x2, x3;
+        f2_unpack(f2_mul(f2_mul(f2_pack(h4.x, h4.y), ff), f2_pack(__uint_as_float(v[j]), __uint_as_float(v[j + 1]))), x0, x1);
+        f2_unpack(f2_mul(f2_mul(f2_pack(h4.z, h4.w), ff), f2_pack(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]))), x2, x3);
+        if (keep != 0xFFFFFFFFu) {
+            x0 = keep & (1u << j) ? x0 : 0.f;
+            x1 = keep & (2u << j) ? x1 : 0.f;
+            x2 = keep & (4u << j) ? x2 : 0.f;
+            x3 = keep & (8u << j) ? x3 : 0.f;
+        }
+        v[j / 2] = pack_bf16(x0, x1);
+        v[j / 2 + 1] = pack_bf16(x2, x3);
+    }
+}
 // One thread of a converged warp. Issuing threads are chosen by this and not by lane index: the compiler
 // then keeps an MMA's descriptors in uniform registers, without which an issue takes 80 cycles and more
 // (measured: 128 x 128 x 16 every 66 cycles against 89, 128 x 64 with A in TMEM 32 against 79).
@@ -249,8 +283,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
         for (int i = 0; i < NBARS; ++i) {
             int n = 1;
             if (i == B_MR || i == B_YF || i == B_SC || (i >= B_RF && i < B_RF + RINGS)) n = 8;
-            if (i == B_PE || i == B_PE + 1) n = kState ? 8 : 16;
-            if (i == B_XE || i == B_XE + 1) n = 8;
+            if (i == B_PE || i == B_PE + 1) n = 16;
+            if (i == B_XE || i == B_XE + 1) n = 16;
             if (i >= B_YS && i < B_YS + 4) n = 4;
             ptx::mbar_init(bar(i), n);
         }
@@ -299,72 +333,115 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
     auto gates = [&](int buf, int s) { return reinterpret_cast<float*>(smem + OFF_GATE + (2 * buf + s) * GATE_BYTES); };
     const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16);  // this warp's TMEM lane quarter
 
-    if (warp < 8) {
-        // ================= M, the scaling of y, the output tile =================
-        if constexpr (!kState) {
-            const int s = warp >> 2, q = warp & 3, i = 32 * q + lane;
-            const uint32_t tm_m = tl + TM_M + 64 * s, tm_y = tl + TM_Y + 64 * s;
-            const int h = slot_head(s), c0 = slot_tile(s), row0 = seg[SEG_ROW];
-            const float D = a.D ? a.D[h] : 0.f;
-            const bool stores = s == 0 || seg[SEG_SECOND];
-            if (nc > 0) {  // blocks right of the diagonal stay zero
-                const uint32_t zero[16] = {};
-                for (int b = q + 1; b < 4; ++b) ptx::tmem_st16(tm_m + 16 * b, zero);
+    // ---- X' pieces (warps 0-15): 32 tokens x 64 channels of X' = w x as three bf16 terms, tokens pt and
+    // pt + 16 in a thread (16 token rows further on the swizzle is the same, so offsets advance by 2 KB).
+    // Pieces 0, 1 of a chunk are formed by warps 0-7, pieces 2, 3 by warps 8-15.
+    const int s = (warp >> 2) & 1, t128 = tid & 127;
+    const uint32_t x_at = row_at(sb + OFF_X + s * PANEL, t128 >> 3) ^ ((t128 & 7) << 4);
+    auto piece = [&](int k, int i) {
+        const uint32_t slot = (uint32_t)i % RINGS;
+        const float* gt = gates(k & 1, s) + GT_W + PIECE * i + (t128 >> 3);
+        uint32_t u[8];
+        const uint32_t from = x_at + (uint32_t)(k & 1) * 2 * PANEL + (uint32_t)i * (PIECE * 128);
+        const uint32_t to = x_at - OFF_X - s * PANEL + OFF_R + s * SUB + slot * RING;
+        ld_shared_v4(from, u[0], u[1], u[2], u[3]);
+        ld_shared_v4(from + 2048, u[4], u[5], u[6], u[7]);
+        const float w0 = gt[0], w1 = gt[16];
+        if (i >= RINGS) warp_wait(B_RE + slot, k);  // the first half's piece has been read
+        else if (k > 0) warp_wait(B_RE + RINGS + slot, k - 1);  // the last chunk's second half
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint64_t ww = t ? f2_pack(w1, w1) : f2_pack(w0, w0);
+            uint32_t hi[4], mid[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t x = u[4 * t + e];
+                const uint64_t v = f2_mul(f2_pack(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u)), ww);
+                float v0, v1, r0, r1, l0, l1;
+                f2_unpack(v, v0, v1);
+                hi[e] = top_halves(v0, v1);
+                const uint64_t r = f2_sub(v, f2_pack(head(v0), head(v1)));
+                f2_unpack(r, r0, r1);
+                mid[e] = top_halves(r0, r1);
+                f2_unpack(f2_sub(r, f2_pack(head(r0), head(r1))), l0, l1);
+                lo[e] = top_halves(l0, l1);
             }
-            for (int k = 0; k < nc; ++k) {
-                const int buf = k & 1;
-                const uint32_t m = (uint32_t)k >> 1;
-                warp_wait(B_PF + buf, m);
+            st_shared_v4(to + 2048 * t, hi[0], hi[1], hi[2], hi[3]);
+            st_shared_v4(to + 2 * SUB + 2048 * t, mid[0], mid[1], mid[2], mid[3]);
+            st_shared_v4(to + 4 * SUB + 2048 * t, lo[0], lo[1], lo[2], lo[3]);
+        }
+        ptx::fence_proxy_async_smem();
+        warp_arrive(B_RF + slot);
+    };
+    // The rows behind the sequence in its last tiles belong to others and may hold anything: zeros, as
+    // their products would otherwise reach valid rows as 0 x NaN. Rows [lo, hi) of this slot's panel.
+    auto zero_rows = [&](uint32_t panel, int lo, int hi) {
+        for (int e = t128; e < (hi - lo) * 8; e += 128) st_shared_v4(row_at(panel, lo + (e >> 3)) ^ ((e & 7) << 4), 0, 0, 0, 0);
+        ptx::fence_proxy_async_smem();
+    };
+
+    if (warp < 8) {
+        // ================= X' (first half), M, the scaling of y =================
+        const int q = warp & 3, i = 32 * q + lane;
+        const uint32_t tm_m = tl + TM_M + 64 * s, tm_y = tl + TM_Y + 64 * s;
+        if (!kState && nc > 0) {  // blocks right of the diagonal stay zero
+            const uint32_t zero[16] = {};
+            for (int b = q + 1; b < 4; ++b) ptx::tmem_st16(tm_m + 16 * b, zero);
+        }
+        auto pieces = [&](int k) {
+            const int valid = min(CH, len - CH * k);
+            warp_wait(B_PF + (k & 1), (uint32_t)k >> 1);
+            warp_wait(B_XF + (k & 1), (uint32_t)k >> 1);
+            if (valid < CH / 2) {
+                zero_rows(sb + OFF_X + (2 * (k & 1) + s) * PANEL, valid, CH / 2);
+                ptx::named_sync(1 + s, 128);
+            }
+#pragma unroll 1
+            for (int i = 0; i < PIECES / 2; ++i) piece(k, i);
+        };
+        if (nc > 0) pieces(0);
+        for (int k = 0; k < nc; ++k) {
+            const int buf = k & 1;
+            if constexpr (!kState) {
                 warp_wait(B_GF, k);
                 ptx::tc_fence_after();
                 const float* gt = gates(buf, s);
                 const float ci = gt[GT_C + i];
                 const float* R = sums + (2 * buf + s) * 4;
-                float before = 0.f;  // sum of a over the blocks between block b and this row's
-                float rowsum[4];
+                // M_ij = G_ij h_j 2^{c_i + (sum of a over the blocks between)}, both factors at most 1
+                float before = 0.f, dist[4];
 #pragma unroll
                 for (int b = 3; b >= 0; --b) {
-                    rowsum[b] = before;
+                    dist[b] = before;
                     if (b < q) before += R[b];
                 }
 #pragma unroll 1
                 for (int b = 0; b < q; ++b) {
-                    float v[32];
-                    ptx::tmem_ld32(tl + TM_G + 32 * b, v);
-                    const float f = ex2f(ci + (b == 0 ? rowsum[0] : b == 1 ? rowsum[1] : rowsum[2]));
-                    const uint64_t ff = f2_pack(f, f);
-                    uint32_t o[16];
+                    uint32_t v[32];
+                    tmem_ld32u(tl + TM_G + 32 * b, v);
+                    const float f = ex2f(ci + (b == 0 ? dist[0] : b == 1 ? dist[1] : dist[2]));
                     ptx::tmem_wait_ld();
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 h4 = ld4(gt + GT_H + 32 * b + j);
-                        float x0, x1;
-                        f2_unpack(f2_mul(f2_mul(f2_pack(h4.x, h4.y), ff), f2_pack(v[j], v[j + 1])), x0, x1);
-                        o[j / 2] = pack_bf16(x0, x1);
-                        f2_unpack(f2_mul(f2_mul(f2_pack(h4.z, h4.w), ff), f2_pack(v[j + 2], v[j + 3])), x0, x1);
-                        o[j / 2 + 1] = pack_bf16(x0, x1);
-                    }
-                    ptx::tmem_st16(tm_m + 16 * b, o);
+                    form_m(v, gt + GT_H + 32 * b, f, 0xFFFFFFFFu);
+                    store16(tm_m + 16 * b, v);
                 }
-                {
-                    float v[32];
-                    ptx::tmem_ld32(tl + TM_G + 32 * q, v);
-                    const uint64_t cc = f2_pack(ci, ci);
-                    uint32_t o[16];
+                {   // the diagonal block: the row factor 2^{c_i - R} undoes h_j's 2^{R - c_j} beyond i
+                    uint32_t v[32];
+                    tmem_ld32u(tl + TM_G + 32 * q, v);
+                    const float Rq = R[q];
                     ptx::tmem_wait_ld();
+                    if (Rq > -100.f) {
+                        form_m(v, gt + GT_H + 32 * q, ex2f(ci - Rq), (2u << lane) - 1u);
+                    } else {  // which fp32 does not hold for decays of more than 2^-100 over 32 tokens
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 c4 = ld4(gt + GT_C + 32 * q + j), d4 = ld4(gt + GT_D + 32 * q + j);
-                        float e0, e1, e2, e3;
-                        f2_unpack(f2_sub(cc, f2_pack(c4.x, c4.y)), e0, e1);
-                        f2_unpack(f2_sub(cc, f2_pack(c4.z, c4.w)), e2, e3);
-                        f2_unpack(f2_mul(f2_mul(f2_pack(ex2f(e0), ex2f(e1)), f2_pack(d4.x, d4.y)), f2_pack(v[j], v[j + 1])), e0, e1);
-                        f2_unpack(f2_mul(f2_mul(f2_pack(ex2f(e2), ex2f(e3)), f2_pack(d4.z, d4.w)), f2_pack(v[j + 2], v[j + 3])), e2, e3);
-                        // a select, not a product with zero: rows behind a sequence may hold anything
-                        o[j / 2] = pack_bf16(j + 0 <= lane ? e0 : 0.f, j + 1 <= lane ? e1 : 0.f);
-                        o[j / 2 + 1] = pack_bf16(j + 2 <= lane ? e2 : 0.f, j + 3 <= lane ? e3 : 0.f);
+                        for (int j = 0; j < 32; j += 2) {
+                            const float2 c2 = *reinterpret_cast<const float2*>(gt + GT_C + 32 * q + j);
+                            const float2 d2 = *reinterpret_cast<const float2*>(gt + GT_D + 32 * q + j);
+                            const float x0 = j <= lane ? __uint_as_float(v[j]) * (ex2f(ci - c2.x) * d2.x) : 0.f;
+                            const float x1 = j + 1 <= lane ? __uint_as_float(v[j + 1]) * (ex2f(ci - c2.y) * d2.y) : 0.f;
+                            v[j / 2] = pack_bf16(x0, x1);
+                        }
                     }
-                    ptx::tmem_st16(tm_m + 16 * q, o);
+                    store16(tm_m + 16 * q, v);
                 }
                 // Y <- e^{c_i} (C S^T), so that M X accumulates onto it
                 const float e = ex2f(ci + before);
@@ -382,57 +459,15 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 ptx::tmem_wait_st();
                 ptx::tc_fence_before();
                 warp_arrive(B_MR);
-                if (lane == 0) ptx::mbar_arrive(bar(B_PE + buf));
-                // ---- output tile: y = Y + D x, in place of x ----
-                warp_wait(B_XF + buf, m);
-                warp_wait(B_YD, k);
-                ptx::tc_fence_after();
-                uint32_t xt = row_at(sb + OFF_X + (2 * buf + s) * PANEL, i);
-                keep_local(xt);
-                const uint64_t dd = f2_pack(D, D);
-                const int valid = min(CH, len - CH * k);
-                const int64_t row = (int64_t)row0 + CH * k + i;
-                __nv_bfloat16* yr = a.y + (row * a.H + h) * a.P + c0;
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    float v[32];
-                    ptx::tmem_ld32(tm_y + 32 * hf, v);
-                    ptx::tmem_wait_ld();
-                    if (hf == 1) {
-                        ptx::tc_fence_before();
-                        warp_arrive(B_YF);
-                    }
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const uint32_t at = xt ^ ((4 * hf + c) << 4);
-                        uint32_t u[4];
-                        ld_shared_v4(at, u[0], u[1], u[2], u[3]);
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) {
-                            float x0, x1;
-                            f2_unpack(f2_fma(f2_pack(__uint_as_float(u[t] << 16), __uint_as_float(u[t] & 0xFFFF0000u)), dd,
-                                             f2_pack(v[8 * c + 2 * t], v[8 * c + 2 * t + 1])),
-                                      x0, x1);
-                            u[t] = pack_bf16(x0, x1);
-                        }
-                        if (valid == CH) {
-                            st_shared_v4(at, u[0], u[1], u[2], u[3]);
-                        } else if (stores && i < valid && c0 + 32 * hf + 8 * c < a.P) {
-                            *reinterpret_cast<uint4*>(yr + 32 * hf + 8 * c) = make_uint4(u[0], u[1], u[2], u[3]);
-                        }
-                    }
-                }
-                if (valid == CH) {
-                    ptx::fence_proxy_async_smem();
-                    warp_arrive(B_YS + 2 * s + buf);
-                }
             }
+            if (lane == 0) ptx::mbar_arrive(bar(B_PE + buf));
+            if (kState && lane == 0) ptx::mbar_arrive(bar(B_XE + buf));
+            if (k + 1 < nc) pieces(k + 1);
         }
     } else if (warp < 16) {
-        // ================= X' and the state =================
-        const int s = (warp >> 2) - 2, n = 32 * (warp & 3) + lane;
-        const int t128 = tid & 127, pt = t128 >> 3, pc = t128 & 7;  // token and 16-byte chunk of a piece
-        const uint32_t tm_s = tl + TM_ST + 64 * s;
+        // ================= the state, the output tile, X' (second half) =================
+        const int n = 32 * (warp & 3) + lane;  // state row, and token row of the output tile
+        const uint32_t tm_s = tl + TM_ST + 64 * s, tm_y = tl + TM_Y + 64 * s;
         if (!idle) {  // entry state: the initial state carried through the earlier segments
             const int c0 = slot_tile(s), seg_first = seg[SEG_FIRST], seg_j = seg[SEG_J], unit = blockIdx.x % p.units;
             const size_t sbase = (((size_t)seg[SEG_SEQ] * a.H + slot_head(s)) * a.P + c0) * a.NS + n;
@@ -466,64 +501,57 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
             }
             ptx::tmem_wait_st();
         }
-        float log_decay = 0.f;
-        // piece i of chunk k: 32 tokens x 64 channels of X' = w x as three bf16 terms, tokens pt and pt + 16
-        // in this thread (16 token rows further on the swizzle is the same, so offsets advance by 2 KB)
-        const uint32_t x_at = sb + OFF_X + s * PANEL + sw_chunk(pt, pc, CH), r_at = sb + OFF_R + s * SUB + sw_chunk(pt, pc, PIECE);
-        auto piece = [&](int k, int i, const float* gt) {
-            const uint32_t use = (uint32_t)(PIECES * k + i) / RINGS, slot = (uint32_t)i % RINGS;
-            uint32_t u[8];
-            const uint32_t from = x_at + (uint32_t)(k & 1) * 2 * PANEL + (uint32_t)i * (PIECE * 128), to = r_at + slot * RING;
-            ld_shared_v4(from, u[0], u[1], u[2], u[3]);
-            ld_shared_v4(from + 2048, u[4], u[5], u[6], u[7]);
-            const float w0 = gt[GT_W + PIECE * i + pt], w1 = gt[GT_W + PIECE * i + pt + 16];
-            if (use > 0) warp_wait(B_RE + slot, use - 1);
+        float D = 0.f, log_decay = 0.f;
+        if (!kState && a.D != nullptr) D = a.D[slot_head(s)];
+        auto output = [&](int k) {  // y = Y + D x, in place of x
+            const int buf = k & 1, valid = min(CH, len - CH * k);
+            warp_wait(B_YD, k);
+            ptx::tc_fence_after();
+            uint32_t xt = row_at(sb + OFF_X + (2 * buf + s) * PANEL, n);
+            keep_local(xt);
+            const uint64_t dd = f2_pack(D, D);
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const uint64_t ww = t ? f2_pack(w1, w1) : f2_pack(w0, w0);
-                uint32_t hi[4], mid[4], lo[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t x = u[4 * t + e];
-                    const uint64_t v = f2_mul(f2_pack(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u)), ww);
-                    float v0, v1, r0, r1, l0, l1;
-                    f2_unpack(v, v0, v1);
-                    hi[e] = top_halves(v0, v1);
-                    const uint64_t r = f2_sub(v, f2_pack(head(v0), head(v1)));
-                    f2_unpack(r, r0, r1);
-                    mid[e] = top_halves(r0, r1);
-                    f2_unpack(f2_sub(r, f2_pack(head(r0), head(r1))), l0, l1);
-                    lo[e] = top_halves(l0, l1);
+            for (int hf = 0; hf < 2; ++hf) {
+                float v[32];
+                ptx::tmem_ld32(tm_y + 32 * hf, v);
+                ptx::tmem_wait_ld();
+                if (hf == 1) {
+                    ptx::tc_fence_before();
+                    warp_arrive(B_YF);
                 }
-                st_shared_v4(to + 2048 * t, hi[0], hi[1], hi[2], hi[3]);
-                st_shared_v4(to + 2 * SUB + 2048 * t, mid[0], mid[1], mid[2], mid[3]);
-                st_shared_v4(to + 4 * SUB + 2048 * t, lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const uint32_t at = xt ^ ((4 * hf + c) << 4);
+                    uint32_t u[4];
+                    ld_shared_v4(at, u[0], u[1], u[2], u[3]);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        float x0, x1;
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(u[t] << 16), __uint_as_float(u[t] & 0xFFFF0000u)), dd,
+                                         f2_pack(v[8 * c + 2 * t], v[8 * c + 2 * t + 1])),
+                                  x0, x1);
+                        u[t] = pack_bf16(x0, x1);
+                    }
+                    st_shared_v4(at, u[0], u[1], u[2], u[3]);
+                }
             }
-            ptx::fence_proxy_async_smem();
-            warp_arrive(B_RF + slot);
+            if (valid == CH) {
+                ptx::fence_proxy_async_smem();
+                warp_arrive(B_YS + 2 * s + buf);
+            } else if (n < valid && (s == 0 || seg[SEG_SECOND])) {  // the rows of a partial tile, each by its thread
+                const int c0 = slot_tile(s);
+                __nv_bfloat16* yr = a.y + (((int64_t)seg[SEG_ROW] + CH * k + n) * a.H + slot_head(s)) * a.P + c0;
+                for (int c = 0; c < 8 && c0 + 8 * c < a.P; ++c) {
+                    uint32_t u[4];
+                    ld_shared_v4(xt ^ (c << 4), u[0], u[1], u[2], u[3]);
+                    *reinterpret_cast<uint4*>(yr + 8 * c) = make_uint4(u[0], u[1], u[2], u[3]);
+                }
+            }
         };
         for (int k = 0; k < nc; ++k) {
-            const int buf = k & 1;
-            const uint32_t m = (uint32_t)k >> 1;
-            const int valid = min(CH, len - CH * k);
-            warp_wait(B_PF + buf, m);
-            warp_wait(B_XF + buf, m);
-            if (valid < CH) {
-                // the rows behind the sequence belong to others and may hold anything: zeros in X and B,
-                // whose products would otherwise reach valid rows as 0 x NaN
-                warp_wait(b_bar(k), b_par(k));
-                for (int e = t128; e < (CH - valid) * 8; e += 128) {
-                    const uint32_t off = sw_chunk(valid + (e >> 3), e & 7, CH);
-                    st_shared_v4(sb + OFF_X + (2 * buf + s) * PANEL + off, 0, 0, 0, 0);
-                    if (s < npanel) st_shared_v4(sb + b_off(k) + s * PANEL + off, 0, 0, 0, 0);
-                }
-                ptx::fence_proxy_async_smem();
-                ptx::named_sync(1 + s, 128);
-            }
-            const float* gt = gates(buf, s);
-#pragma unroll 1
-            for (int i = 0; i < RINGS; ++i) piece(k, i, gt);
+            const int buf = k & 1, valid = min(CH, len - CH * k);
             // the state: bf16 copy as the operand of C S^T, and its decay over this chunk
+            warp_wait(B_PF + buf, (uint32_t)k >> 1);
             if (k > 0) warp_wait(B_SD, k - 1);
             if (!kState && k > 0) warp_wait(B_ID, k - 1);  // the last operand has been read
             ptx::tc_fence_after();
@@ -542,21 +570,29 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                     keep_local(at);
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
-                        st_shared_v4(at ^ ((4 * hf + c) << 4), pack_bits(v[8 * c], v[8 * c + 1]),
-                                     pack_bits(v[8 * c + 2], v[8 * c + 3]), pack_bits(v[8 * c + 4], v[8 * c + 5]),
-                                     pack_bits(v[8 * c + 6], v[8 * c + 7]));
+                        st_shared_v4(at ^ ((4 * hf + c) << 4), pack_bits(v[8 * c], v[8 * c + 1]), pack_bits(v[8 * c + 2], v[8 * c + 3]),
+                                     pack_bits(v[8 * c + 4], v[8 * c + 5]), pack_bits(v[8 * c + 6], v[8 * c + 7]));
                 }
                 scale32(v, dd);
                 ptx::tmem_st32(tm_s + 32 * hf, v);
             }
             ptx::tmem_wait_st();
+            if (valid < CH) {  // before any product of this chunk's state (and of its M X)
+                warp_wait(b_bar(k), b_par(k));
+                if (s < npanel) zero_rows(sb + b_off(k) + s * PANEL, valid, CH);
+                warp_wait(B_XF + buf, (uint32_t)k >> 1);
+                zero_rows(sb + OFF_X + (2 * buf + s) * PANEL, max(valid, CH / 2), CH);
+                ptx::named_sync(3 + s, 128);
+            }
             ptx::fence_proxy_async_smem();
             ptx::tc_fence_before();
             warp_arrive(B_SC);
+            if (!kState && k > 0) output(k - 1);
+            warp_wait(B_XF + buf, (uint32_t)k >> 1);
 #pragma unroll 1
-            for (int i = RINGS; i < PIECES; ++i) piece(k, i, gt);
-            warp_arrive(B_PE + buf);
-            if (kState) warp_arrive(B_XE + buf);
+            for (int i = PIECES / 2; i < PIECES; ++i) piece(k, i);
+            if (lane == 0) ptx::mbar_arrive(bar(B_PE + buf));
+            if (kState && lane == 0) ptx::mbar_arrive(bar(B_XE + buf));
         }
         if (nc > 0) {
             warp_wait(B_SD, nc - 1);
@@ -584,6 +620,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 }
             }
         }
+        if (!kState && nc > 0) output(nc - 1);
     } else if (warp == 16 || warp == 19) {
         // ================= MMA issue (one thread of each warp) =================
         if (elect_one()) {
@@ -609,7 +646,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                             for (int term = 0; term < 3; ++term)
                                 ptx::mma_bf16(tmem + TM_ST, desc(dpanel, b_off(k) + i * (PIECE * 128u) + st * 2048u),
                                               desc(dsub, OFF_R + slot * RING + term * 2 * SUB + st * 2048u), ID_STATE, 1);
-                        ptx::mma_commit(bar(B_RE + slot));
+                        ptx::mma_commit(bar(B_RE + i));  // (i = RINGS * half + slot)
                     }
                     if (dead) break;
                     ptx::mma_commit(bar(B_SD));
@@ -622,8 +659,10 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                     wait(B_CF, k);
                     if (dead) return;
                     ptx::tc_fence_after();
-                    for (int st = 0; st < ks; ++st)
-                        ptx::mma_bf16(tmem + TM_G, desc(d16, OFF_C + kmajor(st)), desc(d16, OFF_B + kmajor(st)), ID_G, st > 0);
+#pragma unroll
+                    for (int st = 0; st < 8; ++st)
+                        if (st < ks)
+                            ptx::mma_bf16(tmem + TM_G, desc(d16, OFF_C + kmajor(st)), desc(d16, OFF_B + kmajor(st)), ID_G, st > 0);
                     ptx::mma_commit(bar(B_GF));
                 };
                 if (nc > 0) issue_g(0);
@@ -632,12 +671,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                     if (k > 0) wait(B_YF, k - 1);
                     if (dead) break;
                     ptx::tc_fence_after();
-                    for (int st = 0; st < ks; ++st)
-                        ptx::mma_bf16(tmem + TM_Y, desc(d16, OFF_C + kmajor(st)), desc(dpanel, OFF_S + st * 2048u), ID_INTER, st > 0);
+#pragma unroll
+                    for (int st = 0; st < 8; ++st)
+                        if (st < ks)
+                            ptx::mma_bf16(tmem + TM_Y, desc(d16, OFF_C + kmajor(st)), desc(dpanel, OFF_S + st * 2048u), ID_INTER, st > 0);
                     ptx::mma_commit(bar(B_ID));
                     wait(B_MR, k);
-                    if (len - CH * k < CH)  // rows of X zeroed behind the sequence's end (before the first piece)
-                        wait(B_RF + RINGS - 1, (uint32_t)(PIECES * k + PIECES - 1) / RINGS);
                     if (dead) break;
                     ptx::tc_fence_after();
 #pragma unroll
