@@ -2,10 +2,13 @@
 //   u = x silu(z);  y = w u rsqrt(mean_group(u^2) + eps)
 // the norm behind a selective scan (gated_rmsnorm.cu has the gate behind the norm, one group a row).
 //
-// Bound: bytes, three streams. A team of threads owns one group of one row: a warp for groups of up
-// to 32 x 4 vectors of 16 bytes, else the block. The team keeps u in registers between the sum of
+// Bound: bytes, three streams. A team of threads owns one group of one row: a warp for groups of up to
+// 64 vectors of 16 bytes, then 64, 128 and 256 threads. The team keeps u in registers between the sum of
 // squares and the store, so x and z are read once; elements beyond the registers (groups wider than
-// the block's 256 x 4 vectors) are read and gated a second time. fp32 math, one rounding at the store.
+// 256 x 8 vectors) are read and gated a second time. Few threads with several vectors each have more loads
+// in flight per synchronisation: 32768 rows of 4096 bf16 take 138 us with 128 threads x 4 vectors, 156 with
+// 256 x 2, 182 with 512 x 1; 8192 rows of 8192 77 us with 128 x 8, 86 with 256 x 2 and re-reads; 16384 rows
+// of 8 groups of 1024 149 us with 64 x 2, 171 with a warp x 4. fp32 math, one rounding at the store.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -15,16 +18,15 @@
 namespace gdn {
 namespace ssm {
 
-constexpr int NORM_THREADS = 256;
-
-template <typename T, int VEC, int TEAM, int KEEP>
-__global__ void __launch_bounds__(NORM_THREADS) group_norm_kernel(const T* __restrict__ x, int64_t xs,
+// Blocks of NT threads hold NT / TEAM teams.
+template <typename T, int VEC, int TEAM, int KEEP, int NT = (TEAM > 32 ? TEAM : 128)>
+__global__ void __launch_bounds__(NT) group_norm_kernel(const T* __restrict__ x, int64_t xs,
                                                                   const T* __restrict__ z, int64_t zs,
                                                                   const T* __restrict__ w, T* __restrict__ y,
                                                                   int64_t units, int C, int groups, float eps) {
-    __shared__ float part[NORM_THREADS / 32];
+    __shared__ float part[NT / 32];
     const int team = threadIdx.x / TEAM, me = threadIdx.x % TEAM;
-    const int64_t unit = (int64_t)blockIdx.x * (NORM_THREADS / TEAM) + team;
+    const int64_t unit = (int64_t)blockIdx.x * (NT / TEAM) + team;
     if (TEAM == 32 && unit >= units) return;  // whole warps; block teams are launched exactly
     const int64_t row = unit / groups;
     const int gs = C / groups, c0 = (int)(unit - row * groups) * gs;
@@ -68,7 +70,7 @@ __global__ void __launch_bounds__(NORM_THREADS) group_norm_kernel(const T* __res
         __syncthreads();
         ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < NORM_THREADS / 32; ++i) ss += part[i];
+        for (int i = 0; i < NT / 32; ++i) ss += part[i];
     }
     const float rstd = rsqrtf(ss / (float)gs + eps);
 #pragma unroll
@@ -91,12 +93,12 @@ __global__ void __launch_bounds__(NORM_THREADS) group_norm_kernel(const T* __res
     }
 }
 
-template <typename T, int VEC, int TEAM, int KEEP>
+template <typename T, int VEC, int TEAM, int KEEP, int NT = (TEAM > 32 ? TEAM : 128)>
 static cudaError_t norm_launch(const void* x, int64_t xs, const void* z, int64_t zs, const void* w, void* y, int64_t units,
                                int C, int groups, float eps, cudaStream_t stream) {
-    const int64_t per = NORM_THREADS / TEAM, blocks = (units + per - 1) / per;
+    const int64_t per = NT / TEAM, blocks = (units + per - 1) / per;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-    group_norm_kernel<T, VEC, TEAM, KEEP><<<(unsigned)blocks, NORM_THREADS, 0, stream>>>(
+    group_norm_kernel<T, VEC, TEAM, KEEP, NT><<<(unsigned)blocks, NT, 0, stream>>>(
         static_cast<const T*>(x), xs, static_cast<const T*>(z), zs, static_cast<const T*>(w), static_cast<T*>(y), units, C,
         groups, eps);
     return cudaGetLastError();
@@ -107,10 +109,15 @@ static cudaError_t norm_vec(const void* x, int64_t xs, const void* z, int64_t zs
                             int groups, float eps, cudaStream_t stream) {
     const int nv = C / groups / VEC;
     const int64_t units = rows * groups;
-    if (nv <= 32) return norm_launch<T, VEC, 32, 1>(x, xs, z, zs, w, y, units, C, groups, eps, stream);
-    if (nv <= 128) return norm_launch<T, VEC, 32, 4>(x, xs, z, zs, w, y, units, C, groups, eps, stream);
-    if (nv <= 512) return norm_launch<T, VEC, 256, 2>(x, xs, z, zs, w, y, units, C, groups, eps, stream);
-    return norm_launch<T, VEC, 256, 4>(x, xs, z, zs, w, y, units, C, groups, eps, stream);
+#define GDN_NORM(TEAM, KEEP) norm_launch<T, VEC, TEAM, KEEP>(x, xs, z, zs, w, y, units, C, groups, eps, stream)
+    if (nv <= 32) return GDN_NORM(32, 1);
+    if (nv <= 64) return GDN_NORM(32, 2);
+    if (nv <= 128) return GDN_NORM(64, 2);
+    if (nv <= 256) return GDN_NORM(128, 2);
+    if (nv <= 512) return GDN_NORM(128, 4);
+    if (nv <= 1024) return GDN_NORM(128, 8);
+    return GDN_NORM(256, 8);
+#undef GDN_NORM
 }
 
 template <typename T>

@@ -23,7 +23,7 @@ __device__ __forceinline__ __half from_float<__half>(float x) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// VEC consecutive elements: one 16-byte access (VEC = 16 / sizeof(T)) or one element (VEC = 1).
+// VEC consecutive elements: one access of 16 or 8 bytes, or one element (VEC = 1).
 template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) Vec {
     T v[VEC];
@@ -33,6 +33,9 @@ __device__ __forceinline__ Vec<T, VEC> ldg(const T* p) {
     Vec<T, VEC> r;
     if constexpr (sizeof(T) * VEC == 16) {
         const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+        r = *reinterpret_cast<const Vec<T, VEC>*>(&u);
+    } else if constexpr (sizeof(T) * VEC == 8) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
         r = *reinterpret_cast<const Vec<T, VEC>*>(&u);
     } else {
 #pragma unroll
@@ -44,6 +47,8 @@ template <typename T, int VEC>
 __device__ __forceinline__ void stg(T* p, const Vec<T, VEC>& r) {
     if constexpr (sizeof(T) * VEC == 16) {
         *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&r);
+    } else if constexpr (sizeof(T) * VEC == 8) {
+        *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(&r);
     } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) p[i] = r.v[i];

@@ -12,21 +12,23 @@ from __future__ import annotations
 import torch
 
 from ._lib import load_library
-from .binding import _check, _same_device, _workspace
+from .binding import _check, _workspace, _ws_cache
 
 __all__ = ["causal_conv_prefill", "causal_conv_prefill_varlen", "causal_conv_decode", "selective_scan_prefill",
            "selective_scan_prefill_varlen", "selective_scan_decode", "gated_group_rmsnorm"]
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+# the current stream's handle without a Stream object: a single-token call is bound by its host time
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _call(dev, what, fn, *args):
-    """fn(*args, stream) on torch's current stream of ``dev``."""
-    if dev.index == torch.cuda.current_device():
-        code = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    """fn(*args, stream) on torch's current stream of device index ``dev``."""
+    if dev == torch.cuda.current_device():
+        code = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            code = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            code = fn(*args, _raw_stream(dev))
     if code:
         _check(code, what)
 
@@ -35,73 +37,102 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
+def _on_one_device(first, *others):
+    """The index of the CUDA device that holds every tensor."""
+    dev = first.get_device()
+    for t in others:
+        if t.get_device() != dev:
+            if dev >= 0 and t.get_device() >= 0:
+                raise ValueError("all tensors must be on the same CUDA device")
+            dev = -1
+    if dev < 0:
+        raise ValueError("all inputs must be CUDA tensors")
+    return dev
+
+
+def _status(dev):
+    """Address of the status word of the device's cached workspace (the one ``read_status`` reads)."""
+    ws = _ws_cache.get(dev)
+    if ws is None:
+        ws = _workspace(torch.device("cuda", dev), 256)
+    return ws.data_ptr()
+
+
 def _rows(t, lead, align=1):
     """(t, row stride in elements): t with its ``lead`` leading dims as evenly spaced rows and its
     other dims contiguous inside a row, t itself where that holds and pointer and stride are
     multiples of ``align`` elements, else a contiguous copy."""
+    shape = t.shape
     width = 1
-    for d in range(t.dim() - 1, lead - 1, -1):
-        if t.shape[d] != 1 and t.stride(d) != width:
-            return _packed_rows(t, lead, align)
-        width *= t.shape[d]
-    stride, rows = None, 1
-    for d in range(lead - 1, -1, -1):
-        if t.shape[d] == 1:
-            continue
-        if stride is None:
-            stride = t.stride(d)
-        elif t.stride(d) != stride * rows:
-            return _packed_rows(t, lead, align)
-        rows *= t.shape[d]
-    if stride is None:  # one row
+    for n in shape[lead:]:
+        width *= n
+    if not t.is_contiguous():
+        strides = t.stride()
+        inner = 1
+        for d in range(len(shape) - 1, lead - 1, -1):
+            if shape[d] != 1 and strides[d] != inner:
+                return _packed_rows(t, width, align)
+            inner *= shape[d]
+        stride, rows = None, 1
+        for d in range(lead - 1, -1, -1):
+            if shape[d] == 1:
+                continue
+            if stride is None:
+                stride = strides[d]
+            elif strides[d] != stride * rows:
+                return _packed_rows(t, width, align)
+            rows *= shape[d]
+        if stride is None:  # one row
+            stride = width
+        if stride < width:
+            return _packed_rows(t, width, align)
+    else:
         stride = width
-    if stride < width or stride % align or t.data_ptr() % (align * t.element_size()):
-        return _packed_rows(t, lead, align)
+    if align > 1 and (stride % align or t.data_ptr() % (align * t.element_size())):
+        return _packed_rows(t, width, align)
     return t, stride
 
 
-def _packed_rows(t, lead, align):
+def _packed_rows(t, width, align):
     t = t.contiguous()
     if t.data_ptr() % (align * t.element_size()):
         t = t.clone()
-    width = 1
-    for n in t.shape[lead:]:
-        width *= n
     return t, width
 
 
 def _vector(t, n, dtype, name, dev):
     if t is None:
         return None
-    if t.dtype != dtype or tuple(t.shape) != (n,):
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name} must be {dtype} of shape [{n}]")
-    if t.device != dev:
+    if t.get_device() != dev:
         raise ValueError("all tensors must be on the same CUDA device")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _initial(s0, shape, dtype, dev):
     """The initial state as a contiguous, 16-byte aligned tensor of ``dtype`` (or None)."""
     if s0 is None:
         return None
-    if tuple(s0.shape) != tuple(shape):
-        raise ValueError(f"initial state must have shape {tuple(shape)}, got {tuple(s0.shape)}")
-    s0 = s0.to(device=dev, dtype=dtype).contiguous()
+    if tuple(s0.shape) != shape:
+        raise ValueError(f"initial state must have shape {shape}, got {tuple(s0.shape)}")
+    if s0.dtype != dtype or s0.get_device() != dev:
+        s0 = s0.to(device=torch.device("cuda", dev), dtype=dtype)
+    s0 = s0.contiguous()
     return s0 if s0.data_ptr() % 16 == 0 else s0.clone()
 
 
 def _offsets(cu_seqlens, dev):
     if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or not cu_seqlens.is_cuda or cu_seqlens.numel() < 1:
         raise ValueError("cu_seqlens must be a 1-D int32 CUDA tensor of at least one element")
-    if cu_seqlens.device != dev:
+    if cu_seqlens.get_device() != dev:
         raise ValueError("all tensors must be on the same CUDA device")
     return cu_seqlens.contiguous()
 
 
 # ---------------------------------------------------------------- causal convolution
 def _check_conv(x, w, bias, packed=False):
-    if not x.is_cuda or not w.is_cuda:
-        raise ValueError("all inputs must be CUDA tensors")
+    dev = _on_one_device(x, w)
     if x.dtype not in _DTYPES or w.dtype != x.dtype:
         raise ValueError("x and w must share dtype fp16, bf16 or fp32")
     if x.dim() != 3 or w.dim() != 2 or w.shape[0] != x.shape[2]:
@@ -112,7 +143,6 @@ def _check_conv(x, w, bias, packed=False):
         raise ValueError("x needs at least one channel")
     if packed and x.shape[0] != 1:
         raise ValueError("varlen inputs are packed: B must be 1")
-    dev = _same_device(x, w)
     return dev, _vector(bias, x.shape[2], x.dtype, "bias", dev)
 
 
@@ -126,10 +156,10 @@ def _conv_prefill(x, w, bias, s0, silu, cu):
     s0 = _initial(s0, (n, W - 1, C), x.dtype, dev)
     x, stride = _rows(x, 2)
     w = w.contiguous()
-    y = torch.empty((B, T, C), dtype=x.dtype, device=dev)
-    sf = torch.empty((n, W - 1, C), dtype=x.dtype, device=dev)
+    y = x.new_empty((B, T, C))
+    sf = x.new_empty((n, W - 1, C))
     _call(dev, "causal_conv_prefill", load_library().causal_conv_prefill, _p(x), stride, _p(w), _p(bias), _p(s0), _p(y),
-          _p(sf), _p(cu), n, T, C, W, int(bool(silu)), _DTYPES[x.dtype])
+          _p(sf), _p(cu), n, T, C, W, bool(silu), _DTYPES[x.dtype])
     return [y, sf]
 
 
@@ -161,20 +191,18 @@ def causal_conv_decode(x, w, state, bias=None, silu: bool = True):
     W = w.shape[1]
     if state.dtype != x.dtype or not state.is_contiguous() or tuple(state.shape) != (B, W - 1, C):
         raise ValueError(f"state must be a contiguous tensor of x's dtype and shape {(B, W - 1, C)}")
-    _same_device(x, state)
+    _on_one_device(x, state)
     x, stride = _rows(x, 2)
     w = w.contiguous()
-    y = torch.empty((B, T, C), dtype=x.dtype, device=dev)
+    y = x.new_empty((B, T, C))
     _call(dev, "causal_conv_decode", load_library().causal_conv_decode, _p(x), stride, _p(w), _p(bias), _p(state), _p(y),
-          B, T, C, W, int(bool(silu)), _DTYPES[x.dtype])
+          B, T, C, W, bool(silu), _DTYPES[x.dtype])
     return y
 
 
 # ---------------------------------------------------------------- selective scan
 def _check_scan(x, dt, A, B, C, D, dt_bias, packed=False):
-    if not (x.is_cuda and dt.is_cuda and A.is_cuda and B.is_cuda and C.is_cuda):
-        raise ValueError("all inputs must be CUDA tensors")
-    dev = _same_device(x, dt, A, B, C)
+    dev = _on_one_device(x, dt, A, B, C)
     if not (x.dtype == B.dtype == C.dtype == torch.bfloat16):
         raise ValueError("x/B/C must be bf16")
     if dt.dtype not in (torch.float32, torch.bfloat16):
@@ -204,15 +232,14 @@ def _scan_prefill(x, dt, A, B, C, D, dt_bias, s0, dt_softplus, cu):
     n = b if cu is None else cu.numel() - 1
     s0 = _initial(s0, (n, H, P, N), torch.float32, dev)
     (x, xs), (dt, dts), (B, bs), (C, cs) = _rows(x, 2, 8), _rows(dt, 2), _rows(B, 2, 8), _rows(C, 2, 8)
-    y = torch.empty((b, T, H, P), dtype=torch.bfloat16, device=dev)
-    sf = torch.empty((n, H, P, N), dtype=torch.float32, device=dev)
+    y = x.new_empty((b, T, H, P))
+    sf = A.new_empty((n, H, P, N))
     lib = load_library()
-    nbytes = lib.selective_scan_scratch_size(n, T, int(cu is not None), H, P, G, N)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    ws = _workspace(dev, 256)  # the status word only
-    _call(dev, "selective_scan_prefill", lib.selective_scan_prefill, _p(x), xs, _p(dt), dts, int(dt.dtype == torch.bfloat16),
-          _p(A), _p(B), bs, _p(C), cs, _p(D), _p(dt_bias), int(bool(dt_softplus)), _p(s0), _p(y), _p(sf), _p(cu), n, T, H, P,
-          G, N, _p(ws), ws.numel(), _p(scratch), nbytes)
+    nbytes = lib.selective_scan_scratch_size(n, T, cu is not None, H, P, G, N)
+    scratch = A.new_empty(nbytes // 4) if nbytes else None
+    _call(dev, "selective_scan_prefill", lib.selective_scan_prefill, _p(x), xs, _p(dt), dts, dt.dtype == torch.bfloat16,
+          _p(A), _p(B), bs, _p(C), cs, _p(D), _p(dt_bias), bool(dt_softplus), _p(s0), _p(y), _p(sf), _p(cu), n, T, H, P,
+          G, N, _status(dev), 256, _p(scratch), nbytes)
     return [y, sf]
 
 
@@ -242,13 +269,13 @@ def selective_scan_decode(x, dt, A, B, C, state, D=None, dt_bias=None, dt_softpl
     dev, (b, T, H, P, G, N), A, D, dt_bias = _check_scan(x, dt, A, B, C, D, dt_bias)
     if state.dtype != torch.float32 or not state.is_contiguous() or tuple(state.shape) != (b, H, P, N):
         raise ValueError("state must be a contiguous fp32 [B, H, P, N] tensor")
-    _same_device(x, state)
+    _on_one_device(x, state)
     if state.data_ptr() % 16:
         raise ValueError("state must be 16-byte aligned")
     (x, xs), (dt, dts), (B, bs), (C, cs) = _rows(x, 2, 8), _rows(dt, 2), _rows(B, 2, 8), _rows(C, 2, 8)
-    y = torch.empty((b, T, H, P), dtype=torch.bfloat16, device=dev)
+    y = x.new_empty((b, T, H, P))
     _call(dev, "selective_scan_decode", load_library().selective_scan_decode, _p(x), xs, _p(dt), dts,
-          int(dt.dtype == torch.bfloat16), _p(A), _p(B), bs, _p(C), cs, _p(D), _p(dt_bias), int(bool(dt_softplus)), _p(state),
+          dt.dtype == torch.bfloat16, _p(A), _p(B), bs, _p(C), cs, _p(D), _p(dt_bias), bool(dt_softplus), _p(state),
           _p(y), b, T, H, P, G, N)
     return y
 
@@ -258,17 +285,15 @@ def gated_group_rmsnorm(x, z, w, groups: int = 1, eps: float = 1e-6):
     """Gated RMSNorm over channel groups with the gate before the norm, over the last dim:
     u = x silu(z); y = w u rsqrt(mean_group(u^2) + eps). x, z [..., C], w [C], all fp16, bf16 or fp32;
     ``groups`` divides C. (``gated_rmsnorm`` has the gate behind the norm.)"""
+    dev = _on_one_device(x, z, w)
     if x.dtype not in _DTYPES or z.dtype != x.dtype or w.dtype != x.dtype:
         raise ValueError("x, z, w must share dtype fp16, bf16 or fp32")
-    if not (x.is_cuda and z.is_cuda and w.is_cuda):
-        raise ValueError("all inputs must be CUDA tensors")
     if x.dim() < 1 or z.shape != x.shape or w.dim() != 1 or w.shape[0] != x.shape[-1]:
         raise ValueError("z must match x and w must be [C]")
     C = x.shape[-1]
     if groups < 1 or C < 1 or C % groups != 0:
         raise ValueError("groups must divide the last dim")
-    dev = _same_device(x, z, w)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = x.new_empty(x.shape)
     (x, xs), (z, zs) = _rows(x, x.dim() - 1), _rows(z, z.dim() - 1)
     w = w.contiguous()
     _call(dev, "gated_group_rmsnorm_forward", load_library().gated_group_rmsnorm_forward, _p(x), xs, _p(z), zs, _p(w), _p(y),
