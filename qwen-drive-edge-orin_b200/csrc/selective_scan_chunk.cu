@@ -4,18 +4,18 @@
 // S <- e^{a_t} S + d_t x_t B_t^T, y_t = S C_t + D x_t is, over one chunk with entry state S,
 //   G      = C B^T                                              [128 x 128]  (shared by the heads of a group)
 //   y      = diag(e^{c}) (C S^T) + M X + D X,   M_ij = G_ij e^{c_i - c_j} d_j for j <= i, else 0
-//   S^T   <- e^{c_L} S^T + B^T X',              X'_j = e^{c_L - c_j} d_j x_j
+//   S     <- e^{c_L} S + X'^T B,                X'_j = e^{c_L - c_j} d_j x_j
 // all four products with 128 rows.
 //
 // A CTA owns one segment of a sequence and two "slots" of a group: a slot is one head's tile of up to
 // 64 channels (a head of 128 is two slots). The two share the B and C tiles and G, and stand side by
-// side in the N = 128 columns of the inter-chunk and state products.
-//   warps 0-7   slot 0 / slot 1: M (bf16) from G into TMEM, the A operand of M X; Y <- e^c Y; the first
-//               half of X', in pieces of 32 tokens into a ring
-//   warps 8-15  slot 0 / slot 1: the state S^T (fp32, TMEM-resident): its bf16 copy (operand of C S^T)
-//               and its decay; the output tile; the second half of X'
-//   warp 16     issues the state products B^T X' (three per piece, below), warp 19 the others, per chunk
-//               inter (C S^T), intra (M X) and the next chunk's G
+// side in the 128 columns of C S^T and the 128 rows of the state.
+//   warps 0-7   M (bf16, both slots) from G in TMEM, in place, the A operand of M X; Y <- e^c Y
+//   warps 8-15  the state S (fp32, TMEM-resident): its bf16 copy (operand of C S^T) and its decay; the
+//               output tile
+//   warps 0-15  X'^T, 32 tokens each warpgroup, into TMEM as the A operand of the state product
+//   warp 16     issues the state products, warp 19 the others, per chunk inter (C S^T), intra (M X) and
+//               the next chunk's G
 //   warp 17     every TMA load and the TMA stores of the output tiles; warp 18 the gates
 //
 // Precision. G and all sums are fp32. M and the state operand of C S^T are rounded to bf16 once (y is
@@ -23,12 +23,14 @@
 // over thousands of tokens: X' is split exactly into three bf16 terms (8 + 8 + 8 bits of an fp32 value),
 // so its products are those of fp32 operands.
 //
-// Decays are kept as base-2 logarithms, relative to 32-token blocks: e^{c_i - c_j} across blocks is
-// a row factor times a column factor, both at most 1 (one exponential per row and block), and inside
-// the diagonal block an exponential per element.
+// Decays are kept as base-2 logarithms, relative to 32-token blocks: e^{c_i - c_j} is a row factor times
+// a column factor, one exponential per row and block. Across blocks both are at most 1; inside a block
+// the row factor undoes the column factor beyond the row, which fp32 holds for decays down to 2^-100.
 //
-// Bound: 32 KB of x and y per slot pair and chunk (5.1 us / 148 at the copy bandwidth) against
-// 3072 tensor cycles.
+// Bound: shared memory, which feeds the MMAs' operands besides everything else (128 bytes a cycle and SM:
+// an MMA of 128 x 128 x 16 with both operands there takes all of it). So the two operands that the warps
+// form, M and X'^T, are in TMEM: with X' in shared memory (8 instead of 4 KB per MMA, and written there)
+// the same chunk took 5.9 K cycles of its bandwidth instead of 4.6 K.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -56,15 +58,11 @@ constexpr int CHUNK_THREADS = 32 * WARPS;
 // ---- shared memory (bytes from a 1024-aligned base); bf16 tiles in the 128-byte swizzle TMA writes:
 // panels of 64 columns, rows of 128 bytes
 constexpr uint32_t PANEL = CH * 128;                 // 16 KB
-constexpr uint32_t OFF_B = 0;                        // 2 panels [128 tokens][64 state]
-constexpr uint32_t OFF_C = OFF_B + 2 * PANEL;        // 2 panels (state pass: the second B buffer)
+constexpr uint32_t OFF_B = 0;                        // 2 buffers x 2 panels [128 tokens][64 state]
+constexpr uint32_t OFF_C = OFF_B + 4 * PANEL;        // 2 panels
 constexpr uint32_t OFF_X = OFF_C + 2 * PANEL;        // 2 buffers x 2 slots [128 tokens][64 channels]; becomes y
-constexpr uint32_t OFF_S = OFF_X + 4 * PANEL;        // 2 slots [128 state][64 channels]
-constexpr uint32_t SUB = PIECE * 128;                // one slot's term of a piece
-constexpr uint32_t RING = 3 * 2 * SUB;               // a piece: 3 terms x 2 slots
-constexpr int RINGS = 2;                             // pieces in the ring
-constexpr uint32_t OFF_R = OFF_S + 2 * PANEL;
-constexpr uint32_t OFF_GATE = OFF_R + RINGS * RING;  // 2 buffers x 2 slots x Gates
+constexpr uint32_t OFF_S = OFF_X + 4 * PANEL;        // 2 panels [128 slot channels][64 state]
+constexpr uint32_t OFF_GATE = OFF_S + 2 * PANEL;     // 2 buffers x 2 slots x Gates
 constexpr uint32_t GATE_BYTES = 4 * CH * 4;
 constexpr uint32_t OFF_MISC = OFF_GATE + 4 * GATE_BYTES;
 constexpr uint32_t MISC_SUMS = 0;                    // block sums [2 buffers][2 slots][4]
@@ -72,7 +70,7 @@ constexpr uint32_t MISC_BAR = 64;
 constexpr uint32_t MISC_TMEM = 344;
 constexpr uint32_t MISC_SEG = 348;                   // the CTA's segment and slots:
 enum { SEG_SEQ, SEG_J, SEG_COUNT, SEG_FIRST, SEG_ROW, SEG_LEN, SEG_HEAD, SEG_TILE = SEG_HEAD + 2, SEG_SECOND = SEG_TILE + 2,
-       SEG_GROUP, SEG_PART, SEG_WORDS };
+       SEG_GROUP, SEG_WORDS };
 constexpr uint32_t MISC_BYTES = 448;
 static_assert(MISC_SEG + 4 * SEG_WORDS <= MISC_BYTES, "segment words overflow");
 constexpr uint32_t CHUNK_SMEM = OFF_MISC + MISC_BYTES + 1024;
@@ -83,10 +81,12 @@ static_assert(CHUNK_SMEM <= 232448, "exceeds the 227 KB per-block shared memory 
 constexpr int GT_C = 0, GT_D = CH, GT_H = 2 * CH, GT_W = 3 * CH;
 
 // ---- TMEM columns (all 128 lanes)
-constexpr uint32_t TM_G = 0;     // G fp32 [token i][token j]
-constexpr uint32_t TM_M = 128;   // M bf16 pairs, 64 columns per slot
-constexpr uint32_t TM_Y = 256;   // y fp32 [token][slot, channel]
-constexpr uint32_t TM_ST = 384;  // S^T fp32 [state][slot, channel]
+constexpr uint32_t TM_G = 0;     // G fp32 [token i][token j]; in place of block b's 32 columns M as bf16
+                                 // pairs, 16 columns per slot
+constexpr uint32_t TM_Y = 128;   // y fp32 [token][slot, channel]
+constexpr uint32_t TM_S = 256;   // S fp32 [slot, channel][state]
+constexpr uint32_t TM_X = 384;   // X'^T bf16 pairs [slot, channel][token]: 2 pieces x 3 terms x 16 columns
+constexpr uint32_t TM_XP = 48;   // columns per piece
 
 // Barriers. *F full, *E empty. A phase is waited for by its parity, so a waiter may neither skip a
 // phase nor let two complete before it looks: every waiter below waits for each phase of its barrier
@@ -94,7 +94,7 @@ constexpr uint32_t TM_ST = 384;  // S^T fp32 [state][slot, channel]
 // phase after.
 enum {
     B_XF = 0, B_XE = 2,  // (XE: state pass)
-    B_BF = 4,            // (two in the state pass)
+    B_BF = 4,
     B_CF = 6,
     B_GF = 7,   // G in TMEM
     B_ID = 8,   // inter product done (y's columns written, C tile free)
@@ -103,21 +103,19 @@ enum {
     B_YF = 11,  // y's columns read
     B_SC = 12,  // state operand written and state decayed
     B_SD = 13,  // state product done
-    B_RF = 14,             // ring of X' pieces: full
-    B_RE = 16,             // empty, per half of the chunk that has been read (each half has its writers)
-    B_PF = 20, B_PE = 22,  // gates
-    B_YS = 24,             // output tile written, per slot and buffer
-    B_DR = 28,             // every MMA of an issuing thread done (exit)
-    B_BE = 30,             // B buffers of the state pass
-    NBARS = 32
+    B_RF = 14, B_RE = 18,  // pieces of X'^T, one pair of barriers per piece of a chunk: written, read
+    B_PF = 22, B_PE = 24,  // gates
+    B_YS = 26,             // output tile written, per slot and buffer
+    B_DR = 30,             // every MMA of an issuing thread done (exit)
+    B_BE = 32,
+    NBARS = 34
 };
-static_assert(PIECES == 2 * RINGS, "a ring holds half a chunk");
 static_assert(MISC_BAR + 8 * NBARS <= MISC_TMEM, "barriers overlap the TMEM address word");
 
 struct ChunkParams {
     CUtensorMap tm_x, tm_b, tm_c, tm_y;
     ScanArgs a;
-    float4* part;      // state pass: final states of segments, [segment][unit][slot][channel / 4][state]
+    float4* part;      // state pass: final states of segments, [segment][unit][state / 4][slot, channel]
     float* part_log;   // and their log2 decays, [segment][unit][slot]
     unsigned int* status;
     int ptiles;        // slots per head
@@ -157,40 +155,70 @@ __device__ __forceinline__ void scale32(uint32_t (&r)[32], uint64_t f) {
         r[j + 1] = __float_as_uint(x1);
     }
 }
-// 16 columns from the first half of a 32-word buffer.
-__device__ __forceinline__ void store16(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
 __device__ __forceinline__ uint32_t pack_bits(uint32_t a, uint32_t b) { return pack_bf16(__uint_as_float(a), __uint_as_float(b)); }
 // Address of a row of a 1024-aligned swizzled panel; its 16-byte chunk c is at that address ^ (c << 4).
 __device__ __forceinline__ uint32_t row_at(uint32_t panel, int row) { return panel + row * 128 + ((row & 7) << 4); }
 // Makes a value opaque here, so that what is derived from it is formed in place and not kept in
 // registers over a loop.
 __device__ __forceinline__ void keep_local(uint32_t& v) { asm volatile("" : "+r"(v)); }
-// v[j] <- bf16 pairs of v[j] h[j] f where bit j of `keep` is set, else 0 (a select, not a product with
-// zero: rows behind a sequence may hold anything).
-__device__ __forceinline__ void form_m(uint32_t (&v)[32], const float* h, float f, uint32_t keep) {
+// log(1 + e^v) = max(v, 0) + log(1 + e), e = e^-|v|, with log(1 + e) = 2 atanh(z), z = e / (2 + e) <= 1/3, by
+// its power series (the first term left out is below 2^-27 of the sum). Accurate relative to the result
+// for any v, in a third of the instructions of log1pf(expf(v)), whose eight copies a chunk the one gate
+// warp has no time for.
+__device__ __forceinline__ float softplus_series(float v) {
+    float x = -fabsf(v);
+    x = x < -200.f ? -200.f : x;  // (NaN stays)
+    const float t = x * LOG2E;
+    const float rest = fmaf(x, 1.9259630e-8f, fmaf(x, LOG2E, -t));  // what the product's and the constant's rounding left out
+    const float e = ex2f(t) * fmaf(rest, 0.69314718f, 1.f);
+    const float z = __fdividef(e, 2.f + e), q = z * z;
+    float s = fmaf(q, 1.f / 15.f, 1.f / 13.f);
+    s = fmaf(q, s, 1.f / 11.f);
+    s = fmaf(q, s, 1.f / 9.f);
+    s = fmaf(q, s, 1.f / 7.f);
+    s = fmaf(q, s, 1.f / 5.f);
+    s = fmaf(q, s, 1.f / 3.f);
+    s = fmaf(q, s, 1.f);
+    return (v > 0.f ? v : 0.f) + 2.f * z * s;
+}
+__device__ __forceinline__ float lds1(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ float4 lds4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ void sts4(uint32_t addr, float4 v) {
+    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+// o <- bf16 pairs of v[j] h[j] f, in a diagonal block only where bit j of `keep` is set, else 0 (a
+// select, not a product with zero: rows behind a sequence may hold anything). h: a shared-memory address.
+template <bool kDiagonal>
+__device__ __forceinline__ void form_m(const uint32_t (&v)[32], uint32_t (&o)[16], uint32_t h, float f, uint32_t keep) {
     const uint64_t ff = f2_pack(f, f);
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
-        const float4 h4 = ld4(h + j);
+        const float4 h4 = lds4(h + 4 * j);
         float x0, x1, x2, x3;
         f2_unpack(f2_mul(f2_mul(f2_pack(h4.x, h4.y), ff), f2_pack(__uint_as_float(v[j]), __uint_as_float(v[j + 1]))), x0, x1);
         f2_unpack(f2_mul(f2_mul(f2_pack(h4.z, h4.w), ff), f2_pack(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]))), x2, x3);
-        if (keep != 0xFFFFFFFFu) {
+        if (kDiagonal) {
             x0 = keep & (1u << j) ? x0 : 0.f;
             x1 = keep & (2u << j) ? x1 : 0.f;
             x2 = keep & (4u << j) ? x2 : 0.f;
             x3 = keep & (8u << j) ? x3 : 0.f;
         }
-        v[j / 2] = pack_bf16(x0, x1);
-        v[j / 2 + 1] = pack_bf16(x2, x3);
+        o[j / 2] = pack_bf16(x0, x1);
+        o[j / 2 + 1] = pack_bf16(x2, x3);
     }
+}
+__device__ __forceinline__ uint32_t ld_shared_u16(uint32_t addr) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
+    return v;
 }
 // One thread of a converged warp. Issuing threads are chosen by this and not by lane index: the compiler
 // then keeps an MMA's descriptors in uniform registers, without which an issue takes 80 cycles and more
@@ -276,13 +304,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
             }
             seg[SEG_SECOND] = second;
             seg[SEG_GROUP] = g;
-            seg[SEG_PART] = blockIdx.x * 2;  // (segment, unit), slot 0
         }
     }
     if (tid == 32) {
         for (int i = 0; i < NBARS; ++i) {
             int n = 1;
-            if (i == B_MR || i == B_YF || i == B_SC || (i >= B_RF && i < B_RF + RINGS)) n = 8;
+            if (i == B_MR || i == B_YF || i == B_SC) n = 8;
+            if (i >= B_RF && i < B_RF + PIECES) n = 4;
             if (i == B_PE || i == B_PE + 1) n = 16;
             if (i == B_XE || i == B_XE + 1) n = 16;
             if (i >= B_YS && i < B_YS + 4) n = 4;
@@ -312,7 +340,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
     // whatever is there (every access stays in its buffer), issuing threads stop.
     bool dead = false;
     auto wait = [&](int b, uint32_t parity) {
-        if (!dead && !ptx::mbar_wait(bar(b), parity & 1u, WAIT_ITERS)) {
+        if (!dead && !ptx::mbar_wait_compact(bar(b), parity & 1u, WAIT_ITERS)) {
             dead = true;
             scan_wait_failed(p.status);
         }
@@ -321,169 +349,105 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
         wait(b, parity);
         __syncwarp();
     };
-    // B tile of chunk k
-    auto b_off = [](int k) { return (kState && (k & 1)) ? OFF_C : OFF_B; };
-    auto b_bar = [](int k) { return kState ? B_BF + (k & 1) : B_BF; };
-    auto b_par = [](int k) { return kState ? (uint32_t)k >> 1 : (uint32_t)k; };
+    auto b_off = [](int k) { return OFF_B + (uint32_t)(k & 1) * 2 * PANEL; };
+    // Warps 0-15: one warp of a warpgroup polls (`f` waits), the others sleep in a named barrier until it has
+    // seen all: twenty polling warps took a third of the issue slots.
+    auto team_wait = [&](auto&& f) {
+        if ((warp & 3) == 0) f();
+        ptx::named_sync(1 + (warp >> 2), 128);
+    };
     auto warp_arrive = [&](int b) {
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar(b));
     };
-    float* sums = reinterpret_cast<float*>(smem + OFF_MISC + MISC_SUMS);
-    auto gates = [&](int buf, int s) { return reinterpret_cast<float*>(smem + OFF_GATE + (2 * buf + s) * GATE_BYTES); };
+    // gates and block sums as shared-memory addresses (plain pointers would load through the generic path)
+    auto gates = [&](int buf, int s) { return sb + OFF_GATE + (uint32_t)(2 * buf + s) * GATE_BYTES; };
+    auto sums = [&](int buf, int s) { return sb + OFF_MISC + MISC_SUMS + (uint32_t)(2 * buf + s) * 16; };
     const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16);  // this warp's TMEM lane quarter
 
-    // ---- X' pieces (warps 0-15): 32 tokens x 64 channels of X' = w x as three bf16 terms, tokens pt and
-    // pt + 16 in a thread (16 token rows further on the swizzle is the same, so offsets advance by 2 KB).
-    // Pieces 0, 1 of a chunk are formed by warps 0-7, pieces 2, 3 by warps 8-15.
-    const int s = (warp >> 2) & 1, t128 = tid & 127;
-    const uint32_t x_at = row_at(sb + OFF_X + s * PANEL, t128 >> 3) ^ ((t128 & 7) << 4);
-    auto piece = [&](int k, int i) {
-        const uint32_t slot = (uint32_t)i % RINGS;
-        const float* gt = gates(k & 1, s) + GT_W + PIECE * i + (t128 >> 3);
-        uint32_t u[8];
-        const uint32_t from = x_at + (uint32_t)(k & 1) * 2 * PANEL + (uint32_t)i * (PIECE * 128);
-        const uint32_t to = x_at - OFF_X - s * PANEL + OFF_R + s * SUB + slot * RING;
-        ld_shared_v4(from, u[0], u[1], u[2], u[3]);
-        ld_shared_v4(from + 2048, u[4], u[5], u[6], u[7]);
-        const float w0 = gt[0], w1 = gt[16];
-        if (i >= RINGS) warp_wait(B_RE + slot, k);  // the first half's piece has been read
-        else if (k > 0) warp_wait(B_RE + RINGS + slot, k - 1);  // the last chunk's second half
+    // ---- X'^T (warps 0-15): warpgroup i forms piece i of a chunk, 32 tokens; a thread one slot channel
+    // (TMEM lane), whose tokens it reads down a column of the x tile (64 contiguous bytes a warp).
+    const int wg = warp >> 2, quarter = warp & 3, row = 32 * quarter + lane;
+    auto piece = [&](int k) {
+        const int s = quarter >> 1, p = row & 63;
+        uint32_t gt = gates(k & 1, s) + 4 * (GT_W + PIECE * wg);
+        // token t of the piece: rows of 128 bytes whose 16-byte chunks are swizzled by t & 7
+        uint32_t at = sb + OFF_X + (2 * (k & 1) + s) * PANEL + PIECE * wg * 128 + ((p >> 3) << 4) + ((p & 7) << 1);
+        uint32_t to = tl + TM_X + TM_XP * (wg & 1);
+        ptx::tc_fence_after();
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+            uint32_t hi[8], mid[8], lo[8];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const uint64_t ww = t ? f2_pack(w1, w1) : f2_pack(w0, w0);
-            uint32_t hi[4], mid[4], lo[4];
+            for (int j = 0; j < 16; j += 4) {
+                const float4 w4 = lds4(gt + 4 * j);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t x = u[4 * t + e];
-                const uint64_t v = f2_mul(f2_pack(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u)), ww);
-                float v0, v1, r0, r1, l0, l1;
-                f2_unpack(v, v0, v1);
-                hi[e] = top_halves(v0, v1);
-                const uint64_t r = f2_sub(v, f2_pack(head(v0), head(v1)));
-                f2_unpack(r, r0, r1);
-                mid[e] = top_halves(r0, r1);
-                f2_unpack(f2_sub(r, f2_pack(head(r0), head(r1))), l0, l1);
-                lo[e] = top_halves(l0, l1);
+                for (int e = 0; e < 4; e += 2) {
+                    const int t = j + e;
+                    const uint32_t x0 = ld_shared_u16((at ^ ((t & 7) << 4)) + t * 128), x1 = ld_shared_u16((at ^ (((t + 1) & 7) << 4)) + (t + 1) * 128);
+                    const uint64_t v = f2_mul(f2_pack(__uint_as_float(x0 << 16), __uint_as_float(x1 << 16)),
+                                              e ? f2_pack(w4.z, w4.w) : f2_pack(w4.x, w4.y));
+                    float v0, v1, r0, r1, l0, l1;
+                    f2_unpack(v, v0, v1);
+                    hi[(j + e) / 2] = top_halves(v0, v1);
+                    const uint64_t r = f2_sub(v, f2_pack(head(v0), head(v1)));
+                    f2_unpack(r, r0, r1);
+                    mid[(j + e) / 2] = top_halves(r0, r1);
+                    f2_unpack(f2_sub(r, f2_pack(head(r0), head(r1))), l0, l1);
+                    lo[(j + e) / 2] = top_halves(l0, l1);
+                }
             }
-            st_shared_v4(to + 2048 * t, hi[0], hi[1], hi[2], hi[3]);
-            st_shared_v4(to + 2 * SUB + 2048 * t, mid[0], mid[1], mid[2], mid[3]);
-            st_shared_v4(to + 4 * SUB + 2048 * t, lo[0], lo[1], lo[2], lo[3]);
+            ptx::tmem_st8(to, hi);
+            ptx::tmem_st8(to + 16, mid);
+            ptx::tmem_st8(to + 32, lo);
+            at += 16 * 128;
+            to += 8;
+            gt += 64;
         }
-        ptx::fence_proxy_async_smem();
-        warp_arrive(B_RF + slot);
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+        warp_arrive(B_RF + wg);
     };
     // The rows behind the sequence in its last tiles belong to others and may hold anything: zeros, as
-    // their products would otherwise reach valid rows as 0 x NaN. Rows [lo, hi) of this slot's panel.
+    // their products would otherwise reach valid rows as 0 x NaN. Rows [lo, hi) of a panel, by one warpgroup.
     auto zero_rows = [&](uint32_t panel, int lo, int hi) {
-        for (int e = t128; e < (hi - lo) * 8; e += 128) st_shared_v4(row_at(panel, lo + (e >> 3)) ^ ((e & 7) << 4), 0, 0, 0, 0);
+        for (int e = tid & 127; e < (hi - lo) * 8; e += 128) st_shared_v4(row_at(panel, lo + (e >> 3)) ^ ((e & 7) << 4), 0, 0, 0, 0);
         ptx::fence_proxy_async_smem();
     };
+    auto zero_x = [&](int k, int valid) {  // this warpgroup's tokens, both slots
+        if (valid >= PIECE * (wg + 1)) return;
+        for (int s = 0; s < 2; ++s) zero_rows(sb + OFF_X + (2 * (k & 1) + s) * PANEL, max(valid, PIECE * wg), PIECE * (wg + 1));
+    };
+    // Both slots of one head (a head of more than 64 channels, or an odd slot run twice): one M for both.
+    const bool twin = seg[SEG_HEAD] == seg[SEG_HEAD + 1];
 
-    if (warp < 8) {
-        // ================= X' (first half), M, the scaling of y =================
-        const int q = warp & 3, i = 32 * q + lane;
-        const uint32_t tm_m = tl + TM_M + 64 * s, tm_y = tl + TM_Y + 64 * s;
-        if (!kState && nc > 0) {  // blocks right of the diagonal stay zero
-            const uint32_t zero[16] = {};
-            for (int b = q + 1; b < 4; ++b) ptx::tmem_st16(tm_m + 16 * b, zero);
-        }
-        auto pieces = [&](int k) {
-            const int valid = min(CH, len - CH * k);
-            warp_wait(B_PF + (k & 1), (uint32_t)k >> 1);
-            warp_wait(B_XF + (k & 1), (uint32_t)k >> 1);
-            if (valid < CH / 2) {
-                zero_rows(sb + OFF_X + (2 * (k & 1) + s) * PANEL, valid, CH / 2);
-                ptx::named_sync(1 + s, 128);
-            }
-#pragma unroll 1
-            for (int i = 0; i < PIECES / 2; ++i) piece(k, i);
-        };
-        if (nc > 0) pieces(0);
-        for (int k = 0; k < nc; ++k) {
-            const int buf = k & 1;
-            if constexpr (!kState) {
-                warp_wait(B_GF, k);
-                ptx::tc_fence_after();
-                const float* gt = gates(buf, s);
-                const float ci = gt[GT_C + i];
-                const float* R = sums + (2 * buf + s) * 4;
-                // M_ij = G_ij h_j 2^{c_i + (sum of a over the blocks between)}, both factors at most 1
-                float before = 0.f, dist[4];
-#pragma unroll
-                for (int b = 3; b >= 0; --b) {
-                    dist[b] = before;
-                    if (b < q) before += R[b];
-                }
-#pragma unroll 1
-                for (int b = 0; b < q; ++b) {
-                    uint32_t v[32];
-                    tmem_ld32u(tl + TM_G + 32 * b, v);
-                    const float f = ex2f(ci + (b == 0 ? dist[0] : b == 1 ? dist[1] : dist[2]));
-                    ptx::tmem_wait_ld();
-                    form_m(v, gt + GT_H + 32 * b, f, 0xFFFFFFFFu);
-                    store16(tm_m + 16 * b, v);
-                }
-                {   // the diagonal block: the row factor 2^{c_i - R} undoes h_j's 2^{R - c_j} beyond i
-                    uint32_t v[32];
-                    tmem_ld32u(tl + TM_G + 32 * q, v);
-                    const float Rq = R[q];
-                    ptx::tmem_wait_ld();
-                    if (Rq > -100.f) {
-                        form_m(v, gt + GT_H + 32 * q, ex2f(ci - Rq), (2u << lane) - 1u);
-                    } else {  // which fp32 does not hold for decays of more than 2^-100 over 32 tokens
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            const float2 c2 = *reinterpret_cast<const float2*>(gt + GT_C + 32 * q + j);
-                            const float2 d2 = *reinterpret_cast<const float2*>(gt + GT_D + 32 * q + j);
-                            const float x0 = j <= lane ? __uint_as_float(v[j]) * (ex2f(ci - c2.x) * d2.x) : 0.f;
-                            const float x1 = j + 1 <= lane ? __uint_as_float(v[j + 1]) * (ex2f(ci - c2.y) * d2.y) : 0.f;
-                            v[j / 2] = pack_bf16(x0, x1);
-                        }
-                    }
-                    store16(tm_m + 16 * q, v);
-                }
-                // Y <- e^{c_i} (C S^T), so that M X accumulates onto it
-                const float e = ex2f(ci + before);
-                const uint64_t ee = f2_pack(e, e);
-                warp_wait(B_ID, k);
-                ptx::tc_fence_after();
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    uint32_t v[32];
-                    tmem_ld32u(tm_y + 32 * hf, v);
-                    ptx::tmem_wait_ld();
-                    scale32(v, ee);
-                    ptx::tmem_st32(tm_y + 32 * hf, v);
-                }
-                ptx::tmem_wait_st();
-                ptx::tc_fence_before();
-                warp_arrive(B_MR);
-            }
-            if (lane == 0) ptx::mbar_arrive(bar(B_PE + buf));
-            if (kState && lane == 0) ptx::mbar_arrive(bar(B_XE + buf));
-            if (k + 1 < nc) pieces(k + 1);
-        }
-    } else if (warp < 16) {
-        // ================= the state, the output tile, X' (second half) =================
-        const int n = 32 * (warp & 3) + lane;  // state row, and token row of the output tile
-        const uint32_t tm_s = tl + TM_ST + 64 * s, tm_y = tl + TM_Y + 64 * s;
-        if (!idle) {  // entry state: the initial state carried through the earlier segments
-            const int c0 = slot_tile(s), seg_first = seg[SEG_FIRST], seg_j = seg[SEG_J], unit = blockIdx.x % p.units;
-            const size_t sbase = (((size_t)seg[SEG_SEQ] * a.H + slot_head(s)) * a.P + c0) * a.NS + n;
+    if (warp < 16) {
+        // Warps 0-7: M and the scaling of y of chunk k, then pieces 0 and 1 of chunk k + 1.
+        // Warps 8-15: the state at chunk k, the output tile of chunk k - 1, then pieces 2 and 3 of chunk k.
+        // One loop and one copy of each part: the kernel is sensitive to instruction fetch.
+        const bool second_half = warp >= 8;
+        const int cols = wg & 1;  // y: slot; state: 64-column panel
+        const uint32_t tm_s = tl + TM_S + 64 * cols, tm_y = tl + TM_Y + 64 * cols;
+        float D = 0.f, log_decay = 0.f;
+        if (!kState && second_half && a.D != nullptr) D = a.D[slot_head(cols)];
+        if (second_half && !idle) {  // entry state: the initial state carried through the earlier segments
+            const int s = quarter >> 1, ch = slot_tile(s) + (row & 63), seg_first = seg[SEG_FIRST], seg_j = seg[SEG_J];
+            const size_t sbase = (((size_t)seg[SEG_SEQ] * a.H + slot_head(s)) * a.P + ch) * a.NS + 64 * cols;
+            const bool inside = !kState && a.s0 != nullptr && ch < a.P;
 #pragma unroll 1
             for (int q4 = 0; q4 < 4; ++q4) {
                 float v[16];
 #pragma unroll
-                for (int c = 0; c < 16; ++c) {
-                    const int ch = 16 * q4 + c;
-                    v[c] = (!kState && a.s0 != nullptr && c0 + ch < a.P && n < a.NS) ? a.s0[sbase + (size_t)ch * a.NS] : 0.f;
+                for (int c = 0; c < 4; ++c) {
+                    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (inside && 64 * cols + 16 * q4 + 4 * c < a.NS) f = *reinterpret_cast<const float4*>(a.s0 + sbase + 16 * q4 + 4 * c);
+                    v[4 * c] = f.x, v[4 * c + 1] = f.y, v[4 * c + 2] = f.z, v[4 * c + 3] = f.w;
                 }
                 if constexpr (!kState) {
                     for (int e = seg_first; e < seg_first + seg_j; ++e) {
-                        const size_t at = ((size_t)e * p.units + unit) * 2 + s;
-                        const float decay = ex2f(p.part_log[at]);
-                        const float4* src = p.part + (at * (TILE / 4) + 4 * q4) * CH + n;
+                        const size_t at = (size_t)e * p.units + blockIdx.x % p.units;
+                        const float decay = ex2f(p.part_log[2 * at + s]);
+                        const float4* src = p.part + (at * 32 + 16 * cols + 4 * q4) * CH + row;
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
                             const float4 f = src[c * CH];
@@ -501,16 +465,14 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
             }
             ptx::tmem_wait_st();
         }
-        float D = 0.f, log_decay = 0.f;
-        if (!kState && a.D != nullptr) D = a.D[slot_head(s)];
         auto output = [&](int k) {  // y = Y + D x, in place of x
-            const int buf = k & 1, valid = min(CH, len - CH * k);
-            warp_wait(B_YD, k);
+            const int buf = k & 1, valid = min(CH, len - CH * k), s = cols;
+            team_wait([&] { wait(B_YD, k); });
             ptx::tc_fence_after();
-            uint32_t xt = row_at(sb + OFF_X + (2 * buf + s) * PANEL, n);
+            uint32_t xt = row_at(sb + OFF_X + (2 * buf + s) * PANEL, row);
             keep_local(xt);
             const uint64_t dd = f2_pack(D, D);
-#pragma unroll
+#pragma unroll 1
             for (int hf = 0; hf < 2; ++hf) {
                 float v[32];
                 ptx::tmem_ld32(tm_y + 32 * hf, v);
@@ -538,9 +500,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
             if (valid == CH) {
                 ptx::fence_proxy_async_smem();
                 warp_arrive(B_YS + 2 * s + buf);
-            } else if (n < valid && (s == 0 || seg[SEG_SECOND])) {  // the rows of a partial tile, each by its thread
+            } else if (row < valid && (s == 0 || seg[SEG_SECOND])) {  // the rows of a partial tile, each by its thread
                 const int c0 = slot_tile(s);
-                __nv_bfloat16* yr = a.y + (((int64_t)seg[SEG_ROW] + CH * k + n) * a.H + slot_head(s)) * a.P + c0;
+                __nv_bfloat16* yr = a.y + (((int64_t)seg[SEG_ROW] + CH * k + row) * a.H + slot_head(s)) * a.P + c0;
                 for (int c = 0; c < 8 && c0 + 8 * c < a.P; ++c) {
                     uint32_t u[4];
                     ld_shared_v4(xt ^ (c << 4), u[0], u[1], u[2], u[3]);
@@ -548,121 +510,211 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 }
             }
         };
-        for (int k = 0; k < nc; ++k) {
-            const int buf = k & 1, valid = min(CH, len - CH * k);
-            // the state: bf16 copy as the operand of C S^T, and its decay over this chunk
-            warp_wait(B_PF + buf, (uint32_t)k >> 1);
-            if (k > 0) warp_wait(B_SD, k - 1);
-            if (!kState && k > 0) warp_wait(B_ID, k - 1);  // the last operand has been read
-            ptx::tc_fence_after();
-            const float* R = sums + (2 * buf + s) * 4;
-            const float total = (R[0] + R[1]) + (R[2] + R[3]);
-            log_decay += total;
-            const float decay = ex2f(total);
-            const uint64_t dd = f2_pack(decay, decay);
 #pragma unroll 1
-            for (int hf = 0; hf < 2; ++hf) {
-                uint32_t v[32];
-                tmem_ld32u(tm_s + 32 * hf, v);
-                ptx::tmem_wait_ld();
-                if constexpr (!kState) {
-                    uint32_t at = row_at(sb + OFF_S + s * PANEL, n);
-                    keep_local(at);
+        for (int k = second_half ? 0 : -1; k < nc + (second_half ? 1 : 0); ++k) {
+            const int buf = k & 1;
+            if (second_half) {
+                const int valid = min(CH, len - CH * k);
+                if (k < nc) {
+                    // the state: bf16 copy as the operand of C S^T, and its decay over this chunk
+                    team_wait([&] {
+                        wait(B_PF + buf, (uint32_t)k >> 1);
+                        if (k > 0) wait(B_SD, k - 1);
+                        if (!kState && k > 0) wait(B_ID, k - 1);  // the last operand has been read
+                    });
+                    ptx::tc_fence_after();
+                    if (cols < npanel) {
+                        const float4 R = lds4(sums(buf, quarter >> 1));
+                        const float total = (R.x + R.y) + (R.z + R.w);
+                        log_decay += total;
+                        const float decay = ex2f(total);
+                        const uint64_t dd = f2_pack(decay, decay);
+#pragma unroll 1
+                        for (int hf = 0; hf < 2; ++hf) {
+                            uint32_t v[32];
+                            tmem_ld32u(tm_s + 32 * hf, v);
+                            ptx::tmem_wait_ld();
+                            if constexpr (!kState) {
+                                uint32_t at = row_at(sb + OFF_S + cols * PANEL, row);
+                                keep_local(at);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        st_shared_v4(at ^ ((4 * hf + c) << 4), pack_bits(v[8 * c], v[8 * c + 1]), pack_bits(v[8 * c + 2], v[8 * c + 3]),
-                                     pack_bits(v[8 * c + 4], v[8 * c + 5]), pack_bits(v[8 * c + 6], v[8 * c + 7]));
+                                for (int c = 0; c < 4; ++c)
+                                    st_shared_v4(at ^ ((4 * hf + c) << 4), pack_bits(v[8 * c], v[8 * c + 1]), pack_bits(v[8 * c + 2], v[8 * c + 3]),
+                                                 pack_bits(v[8 * c + 4], v[8 * c + 5]), pack_bits(v[8 * c + 6], v[8 * c + 7]));
+                            }
+                            scale32(v, dd);
+                            ptx::tmem_st32(tm_s + 32 * hf, v);
+                        }
+                        ptx::tmem_wait_st();
+                    }
+                    if (valid < CH) {  // before any product of this chunk's state (and of its M X)
+                        team_wait([&] {
+                            wait(B_BF + buf, (uint32_t)k >> 1);
+                            wait(B_XF + buf, (uint32_t)k >> 1);
+                        });
+                        if (cols < npanel) zero_rows(sb + b_off(k) + cols * PANEL, valid, CH);
+                        zero_x(k, valid);
+                    }
+                    ptx::fence_proxy_async_smem();
+                    ptx::tc_fence_before();
+                    warp_arrive(B_SC);
+                } else if (nc > 0) {
+                    team_wait([&] { wait(B_SD, nc - 1); });
+                    ptx::tc_fence_after();
                 }
-                scale32(v, dd);
-                ptx::tmem_st32(tm_s + 32 * hf, v);
-            }
-            ptx::tmem_wait_st();
-            if (valid < CH) {  // before any product of this chunk's state (and of its M X)
-                warp_wait(b_bar(k), b_par(k));
-                if (s < npanel) zero_rows(sb + b_off(k) + s * PANEL, valid, CH);
-                warp_wait(B_XF + buf, (uint32_t)k >> 1);
-                zero_rows(sb + OFF_X + (2 * buf + s) * PANEL, max(valid, CH / 2), CH);
-                ptx::named_sync(3 + s, 128);
-            }
-            ptx::fence_proxy_async_smem();
-            ptx::tc_fence_before();
-            warp_arrive(B_SC);
-            if (!kState && k > 0) output(k - 1);
-            warp_wait(B_XF + buf, (uint32_t)k >> 1);
+                if (!kState && k > 0) output(k - 1);
+            } else if (k >= 0) {
+                const int q = quarter;
+                if constexpr (!kState) {
+                    team_wait([&] { wait(B_GF, k); });
+                    ptx::tc_fence_after();
+                    // M_ij = G_ij h_j 2^{c_i + (sum of a over the blocks between)}: blocks 0, 2 of this warp's
+                    // rows here, 1, 3 in the warp of the other group on the same TMEM lanes
 #pragma unroll 1
-            for (int i = PIECES / 2; i < PIECES; ++i) piece(k, i);
-            if (lane == 0) ptx::mbar_arrive(bar(B_PE + buf));
-            if (kState && lane == 0) ptx::mbar_arrive(bar(B_XE + buf));
+                    for (int b = wg; b < 4; b += 2) {
+                        uint32_t v[32];
+                        const uint32_t at = tl + TM_G + 32 * b;
+                        if (b > q) {  // right of the diagonal
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = 0;
+                            ptx::tmem_st32(at, v);
+                            continue;
+                        }
+                        tmem_ld32u(at, v);
+                        ptx::tmem_wait_ld();
+#pragma unroll 1
+                        for (int s = 0; s < (twin ? 1 : 2); ++s) {
+                            const uint32_t gt = gates(buf, s), R = sums(buf, s);
+                            const float ci = lds1(gt + 4 * (GT_C + row)), Rq = lds1(R + 4 * q);
+                            uint32_t o[16];
+                            if (b < q) {
+                                float e = ci;
+#pragma unroll 1
+                                for (int m = b + 1; m < q; ++m) e += lds1(R + 4 * m);
+                                form_m<false>(v, o, gt + 4 * (GT_H + 32 * b), ex2f(e), 0);
+                            } else if (Rq > -100.f) {  // the row factor undoes h_j's 2^{R - c_j} beyond i
+                                form_m<true>(v, o, gt + 4 * (GT_H + 32 * b), ex2f(ci - Rq), (2u << lane) - 1u);
+                            } else {  // decays beyond fp32's range inside the block: an exponential per element
+#pragma unroll
+                                for (int j = 0; j < 32; j += 4) {
+                                    const float4 c4 = lds4(gt + 4 * (GT_C + 32 * q + j)), d4 = lds4(gt + 4 * (GT_D + 32 * q + j));
+                                    const float x0 = j <= lane ? __uint_as_float(v[j]) * (ex2f(ci - c4.x) * d4.x) : 0.f;
+                                    const float x1 = j + 1 <= lane ? __uint_as_float(v[j + 1]) * (ex2f(ci - c4.y) * d4.y) : 0.f;
+                                    const float x2 = j + 2 <= lane ? __uint_as_float(v[j + 2]) * (ex2f(ci - c4.z) * d4.z) : 0.f;
+                                    const float x3 = j + 3 <= lane ? __uint_as_float(v[j + 3]) * (ex2f(ci - c4.w) * d4.w) : 0.f;
+                                    o[j / 2] = pack_bf16(x0, x1);
+                                    o[j / 2 + 1] = pack_bf16(x2, x3);
+                                }
+                            }
+                            ptx::tmem_st16(at + 16 * s, o);
+                        }
+                    }
+                    // Y <- e^{c_i} (C S^T), so that M X accumulates onto it
+                    float e = lds1(gates(buf, wg) + 4 * (GT_C + row));
+#pragma unroll 1
+                    for (int m = 0; m < q; ++m) e += lds1(sums(buf, wg) + 4 * m);
+                    e = ex2f(e);
+                    const uint64_t ee = f2_pack(e, e);
+                    team_wait([&] { wait(B_ID, k); });
+                    ptx::tc_fence_after();
+#pragma unroll 1
+                    for (int hf = 0; hf < 2; ++hf) {
+                        uint32_t v[32];
+                        tmem_ld32u(tm_y + 32 * hf, v);
+                        ptx::tmem_wait_ld();
+                        scale32(v, ee);
+                        ptx::tmem_st32(tm_y + 32 * hf, v);
+                    }
+                    ptx::tmem_wait_st();
+                    ptx::tc_fence_before();
+                    warp_arrive(B_MR);
+                }
+                if (lane == 0) {
+                    ptx::mbar_arrive(bar(B_PE + buf));
+                    if (kState) ptx::mbar_arrive(bar(B_XE + buf));
+                }
+            }
+            const int kp = second_half ? k : k + 1;
+            if (kp < nc) {
+                team_wait([&] {
+                    if (!second_half) wait(B_PF + (kp & 1), (uint32_t)kp >> 1);
+                    wait(B_XF + (kp & 1), (uint32_t)kp >> 1);
+                    // the piece's columns: read by the products of the piece two before it
+                    if (second_half) wait(B_RE + wg - 2, kp);
+                    else if (kp > 0) wait(B_RE + wg + 2, kp - 1);
+                });
+                if (len - CH * kp < CH) {
+                    if (!second_half) zero_x(kp, len - CH * kp);
+                    ptx::named_sync(1 + wg, 128);
+                }
+                piece(kp);
+                if (second_half && lane == 0) {
+                    ptx::mbar_arrive(bar(B_PE + buf));
+                    if (kState) ptx::mbar_arrive(bar(B_XE + buf));
+                }
+            }
         }
-        if (nc > 0) {
-            warp_wait(B_SD, nc - 1);
-            ptx::tc_fence_after();
-        }
-        if (!idle && (kState || seg[SEG_J] == seg[SEG_COUNT] - 1)) {
-            const int c0 = slot_tile(s);
-            const bool stores = s == 0 || seg[SEG_SECOND];
-            const size_t sbase = (((size_t)seg[SEG_SEQ] * a.H + slot_head(s)) * a.P + c0) * a.NS + n;
-            const size_t at = (size_t)seg[SEG_PART] + s;
-            if (kState && n == 0) p.part_log[at] = log_decay;
+        if (second_half && !idle && (kState || seg[SEG_J] == seg[SEG_COUNT] - 1)) {
+            const int s = quarter >> 1, ch = slot_tile(s) + (row & 63);
+            const size_t sbase = (((size_t)seg[SEG_SEQ] * a.H + slot_head(s)) * a.P + ch) * a.NS + 64 * cols;
+            const bool inside = ch < a.P && (s == 0 || seg[SEG_SECOND]);
+            if (kState && cols == 0 && (row & 63) == 0) p.part_log[2 * (size_t)blockIdx.x + s] = log_decay;
 #pragma unroll 1
             for (int q4 = 0; q4 < 4; ++q4) {
                 float v[16];
                 ptx::tmem_ld16(tm_s + 16 * q4, v);
                 ptx::tmem_wait_ld();
-                if (kState) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        p.part[(at * (TILE / 4) + 4 * q4 + c) * CH + n] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-                } else if (stores && n < a.NS) {
-#pragma unroll
-                    for (int c = 0; c < 16; ++c)
-                        if (c0 + 16 * q4 + c < a.P) a.sf[sbase + (size_t)(16 * q4 + c) * a.NS] = v[c];
+                for (int c = 0; c < 4; ++c) {
+                    const float4 f = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+                    if (kState)
+                        p.part[((size_t)blockIdx.x * 32 + 16 * cols + 4 * q4 + c) * CH + row] = f;
+                    else if (inside && 64 * cols + 16 * q4 + 4 * c < a.NS)
+                        *reinterpret_cast<float4*>(a.sf + sbase + 16 * q4 + 4 * c) = f;
                 }
             }
         }
-        if (!kState && nc > 0) output(nc - 1);
     } else if (warp == 16 || warp == 19) {
         // ================= MMA issue (one thread of each warp) =================
         if (elect_one()) {
-            constexpr uint32_t ID_G = ptx::idesc_bf16(128, 128, 0, 0, 0);      // C B^T
-            constexpr uint32_t ID_INTER = ptx::idesc_bf16(128, 128, 0, 1, 0);  // C S^T       (B MN-major)
-            constexpr uint32_t ID_STATE = ptx::idesc_bf16(128, 128, 1, 1, 0);  // B^T X'      (both MN-major)
+            constexpr uint32_t ID_G = ptx::idesc_bf16(128, 128, 0, 0, 0);      // C B^T, C S^T
             constexpr uint32_t ID_INTRA = ptx::idesc_bf16(128, 64, 0, 1, 0);   // M X         (A in TMEM, B MN-major)
-            const uint32_t d16 = ptx::sw128_desc_lo(sb, 16), dpanel = ptx::sw128_desc_lo(sb, PANEL), dsub = ptx::sw128_desc_lo(sb, SUB);
+            constexpr uint32_t ID_TWIN = ptx::idesc_bf16(128, 128, 0, 1, 0);   // M X of both slots
+            const uint32_t d16 = ptx::sw128_desc_lo(sb, 16), dpanel = ptx::sw128_desc_lo(sb, PANEL);
             auto desc = [](uint32_t base, uint32_t off) { return ptx::desc_pair(base + (off >> 4), ptx::sw128_desc_hi(1024)); };
             auto kmajor = [](int st) { return (uint32_t)(st >> 2) * PANEL + (uint32_t)(st & 3) * 32u; };
+            const int ks = (a.NS + 15) / 16;  // 16-column steps of the state dimension
             if (warp == 16) {
+                const uint32_t id_state = ptx::idesc_bf16(128, 16 * ks, 0, 1, 0);  // X'^T B  (A in TMEM, B MN-major)
                 for (int k = 0; k < nc; ++k) {
-                    wait(b_bar(k), b_par(k));
+                    wait(B_BF + (k & 1), (uint32_t)k >> 1);
                     wait(B_SC, k);
-                    for (int i = 0; i < PIECES && !dead; ++i) {
-                        const uint32_t use = (uint32_t)(PIECES * k + i) / RINGS, slot = (uint32_t)i % RINGS;
-                        wait(B_RF + slot, use);
+#pragma unroll 1
+                    for (int i = 0; i < PIECES; ++i) {
+                        wait(B_RF + i, k);
                         if (dead) break;
                         ptx::tc_fence_after();
 #pragma unroll
                         for (int st = 0; st < PIECE / 16; ++st)
 #pragma unroll
                             for (int term = 0; term < 3; ++term)
-                                ptx::mma_bf16(tmem + TM_ST, desc(dpanel, b_off(k) + i * (PIECE * 128u) + st * 2048u),
-                                              desc(dsub, OFF_R + slot * RING + term * 2 * SUB + st * 2048u), ID_STATE, 1);
-                        ptx::mma_commit(bar(B_RE + i));  // (i = RINGS * half + slot)
+                                ptx::mma_bf16_ts(tmem + TM_S, tmem + TM_X + TM_XP * (i & 1) + 16 * term + 8 * st,
+                                                 desc(dpanel, b_off(k) + (uint32_t)(PIECE * i + 16 * st) * 128u), id_state, 1);
+                        ptx::mma_commit(bar(B_RE + i));
                     }
                     if (dead) break;
                     ptx::mma_commit(bar(B_SD));
-                    if (kState) ptx::mma_commit(bar(B_BE + (k & 1)));
+                    ptx::mma_commit(bar(B_BE + (k & 1)));
                 }
             } else if (!kState) {
-                const int ks = (a.NS + 15) / 16;  // K steps over the state dimension
                 auto issue_g = [&](int k) {
-                    wait(B_BF, k);
+                    wait(B_BF + (k & 1), (uint32_t)k >> 1);
                     wait(B_CF, k);
                     if (dead) return;
                     ptx::tc_fence_after();
-#pragma unroll
-                    for (int st = 0; st < 8; ++st)
-                        if (st < ks)
-                            ptx::mma_bf16(tmem + TM_G, desc(d16, OFF_C + kmajor(st)), desc(d16, OFF_B + kmajor(st)), ID_G, st > 0);
+#pragma unroll 2
+                    for (int st = 0; st < ks; ++st)
+                            ptx::mma_bf16(tmem + TM_G, desc(d16, OFF_C + kmajor(st)), desc(d16, b_off(k) + kmajor(st)), ID_G, st > 0);
                     ptx::mma_commit(bar(B_GF));
                 };
                 if (nc > 0) issue_g(0);
@@ -671,21 +723,28 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                     if (k > 0) wait(B_YF, k - 1);
                     if (dead) break;
                     ptx::tc_fence_after();
-#pragma unroll
-                    for (int st = 0; st < 8; ++st)
-                        if (st < ks)
-                            ptx::mma_bf16(tmem + TM_Y, desc(d16, OFF_C + kmajor(st)), desc(dpanel, OFF_S + st * 2048u), ID_INTER, st > 0);
+#pragma unroll 2
+                    for (int st = 0; st < ks; ++st)
+                            ptx::mma_bf16(tmem + TM_Y, desc(d16, OFF_C + kmajor(st)), desc(d16, OFF_S + kmajor(st)), ID_G, st > 0);
                     ptx::mma_commit(bar(B_ID));
                     wait(B_MR, k);
                     if (dead) break;
                     ptx::tc_fence_after();
-#pragma unroll
-                    for (int s = 0; s < 2; ++s)
-#pragma unroll
+                    const uint32_t xo = OFF_X + (uint32_t)(k & 1) * 2 * PANEL;
+                    if (twin) {
+#pragma unroll 2
                         for (int st = 0; st < CH / 16; ++st)
-                            ptx::mma_bf16_ts(tmem + TM_Y + 64 * s, tmem + TM_M + 64 * s + 8 * st,
-                                             desc(d16, OFF_X + (2 * (k & 1) + s) * PANEL + st * 2048u), ID_INTRA, 1);
+                            ptx::mma_bf16_ts(tmem + TM_Y, tmem + TM_G + 32 * (st >> 1) + 8 * (st & 1), desc(dpanel, xo + st * 2048u), ID_TWIN, 1);
+                    } else {
+#pragma unroll 1
+                        for (int s = 0; s < 2; ++s)
+#pragma unroll 2
+                            for (int st = 0; st < CH / 16; ++st)
+                                ptx::mma_bf16_ts(tmem + TM_Y + 64 * s, tmem + TM_G + 32 * (st >> 1) + 16 * s + 8 * (st & 1),
+                                                 desc(d16, xo + s * PANEL + st * 2048u), ID_INTRA, 1);
+                    }
                     ptx::mma_commit(bar(B_YD));
+                    wait(B_YD, k);  // M has been read: G takes its place
                     if (k + 1 < nc) issue_g(k + 1);
                     if (dead) break;
                 }
@@ -710,9 +769,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
             auto load_b = [&](int k) {
                 if (dead || k >= nc) return;
                 ++nb;
-                ptx::mbar_arrive_expect_tx(bar(b_bar(k)), npanel * PANEL);
+                ptx::mbar_arrive_expect_tx(bar(B_BF + (k & 1)), npanel * PANEL);
                 for (int c = 0; c < npanel; ++c)
-                    ptx::tma_load_4d(sb + b_off(k) + c * PANEL, &p.tm_b, bar(b_bar(k)), 64 * c, g, row0 + CH * k, 0);
+                    ptx::tma_load_4d(sb + b_off(k) + c * PANEL, &p.tm_b, bar(B_BF + (k & 1)), 64 * c, g, row0 + CH * k, 0);
             };
             auto load_c = [&](int k) {
                 if (dead || k >= nc) return;
@@ -731,8 +790,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
             load_x(0);
             load_b(0);
             if (!kState) load_c(0);
-            if (kState) load_b(1);
             load_x(1);
+            load_b(1);
             for (int k = 0; k < nc && !dead; ++k) {
                 if constexpr (kState) {
                     wait(B_XE + (k & 1), (uint32_t)k >> 1);
@@ -740,17 +799,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                     wait(B_BE + (k & 1), (uint32_t)k >> 1);
                     load_b(k + 2);
                 } else {
-                    if (k + 1 < nc) {  // the next tiles on their way to L2 while their buffers are in use
-                        for (int c = 0; c < npanel; ++c) {
-                            ptx::tma_prefetch_4d(&p.tm_b, 64 * c, g, row0 + CH * (k + 1), 0);
-                            ptx::tma_prefetch_4d(&p.tm_c, 64 * c, g, row0 + CH * (k + 1), 0);
-                        }
-                    }
-                    wait(B_ID, k);
+                    if (k + 1 < nc)  // the next C tile on its way to L2 while its buffer is in use
+                        for (int c = 0; c < npanel; ++c) ptx::tma_prefetch_4d(&p.tm_c, 64 * c, g, row0 + CH * (k + 1), 0);
+                    wait(B_ID, k);  // (behind it, by the same thread, G of this chunk: B is free with the state product)
                     load_c(k + 1);
-                    wait(B_SD, k);
-                    wait(B_GF, k);
-                    load_b(k + 1);
+                    wait(B_BE + (k & 1), (uint32_t)k >> 1);
+                    load_b(k + 2);
                     if (len - CH * k >= CH) {  // a full tile: out by TMA (the warps store a partial one themselves)
                         const int buf = k & 1, row = row0 + CH * k;
                         wait(B_YS + buf, (uint32_t)k >> 1);
@@ -766,10 +820,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
             const bool failed = dead;
             dead = false;
             for (int buf = 0; buf < 2; ++buf) {
-                if (kState && nb > buf) wait(B_BF + buf, (uint32_t)(nb - 1 - buf) >> 1);
+                if (nb > buf) wait(B_BF + buf, (uint32_t)(nb - 1 - buf) >> 1);
                 if (nx > buf) wait(B_XF + buf, (uint32_t)(nx - 1 - buf) >> 1);
             }
-            if (!kState && nb > 0) wait(B_BF, (uint32_t)(nb - 1));
             if (ncl > 0) wait(B_CF, (uint32_t)(ncl - 1));
             ptx::bulk_wait_all();
             dead |= failed;
@@ -800,19 +853,25 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float v = next[s][i] + bias[s];
-                    if (a.softplus) v = softplus(v);
+                    if (a.softplus) v = softplus_series(v);
                     d[s][i] = 4 * lane + i < valid ? v : 0.f;
                 }
             if (k + 1 < nc) load(k + 1);
             if (k >= 2) warp_wait(B_PE + buf, ((uint32_t)k >> 1) - 1);
 #pragma unroll
+            for (int s = 0; s < 2; ++s)
+                sts4(gates(buf, s) + 4 * (GT_D + 4 * lane), make_float4(d[s][0], d[s][1], d[s][2], d[s][3]));
+#pragma unroll 1
             for (int s = 0; s < 2; ++s) {
+                const uint32_t gt = gates(buf, s) + 16 * lane;
+                const float4 d4 = lds4(gt + 4 * GT_D);
+                const float A2s = s ? A2[1] : A2[0];
                 // log2 decays; the clamp keeps sums of 128 finite, and 2^-1e30 is zero as well
-                float t[4], pre[4], suf[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) t[i] = fmaxf(d[s][i] * A2[s], -1e30f);
-                pre[0] = t[0], pre[1] = t[0] + t[1], pre[2] = pre[1] + t[2], pre[3] = pre[2] + t[3];
-                suf[3] = 0.f, suf[2] = t[3], suf[1] = t[3] + t[2], suf[0] = suf[1] + t[1];
+                float pre[4], suf[4];
+                const float t0 = fmaxf(d4.x * A2s, -1e30f), t1 = fmaxf(d4.y * A2s, -1e30f), t2 = fmaxf(d4.z * A2s, -1e30f),
+                            t3 = fmaxf(d4.w * A2s, -1e30f);
+                pre[0] = t0, pre[1] = t0 + t1, pre[2] = pre[1] + t2, pre[3] = pre[2] + t3;
+                suf[3] = 0.f, suf[2] = t3, suf[1] = t3 + t2, suf[0] = suf[1] + t1;
                 // sums over the 8 lanes of a 32-token block, from the left and, for the accuracy of the
                 // short distances, from the right
                 float inc = pre[3], dec = pre[3];
@@ -833,15 +892,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 for (int b = 3; b > 0; --b)
                     if (b > (lane >> 3)) behind += R[b];
                 const float f = ex2f(behind);
-                float hv[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) hv[i] = ex2f(right + suf[i]) * d[s][i];
-                float* gt = gates(buf, s) + 4 * lane;
-                *reinterpret_cast<float4*>(gt + GT_C) = make_float4(left + pre[0], left + pre[1], left + pre[2], left + pre[3]);
-                *reinterpret_cast<float4*>(gt + GT_D) = make_float4(d[s][0], d[s][1], d[s][2], d[s][3]);
-                *reinterpret_cast<float4*>(gt + GT_H) = make_float4(hv[0], hv[1], hv[2], hv[3]);
-                *reinterpret_cast<float4*>(gt + GT_W) = make_float4(hv[0] * f, hv[1] * f, hv[2] * f, hv[3] * f);
-                if (lane == 0) *reinterpret_cast<float4*>(sums + (2 * buf + s) * 4) = make_float4(R[0], R[1], R[2], R[3]);
+                const float hv[4] = {ex2f(right + suf[0]) * d4.x, ex2f(right + suf[1]) * d4.y, ex2f(right + suf[2]) * d4.z,
+                                     ex2f(right + suf[3]) * d4.w};
+                sts4(gt + 4 * GT_C, make_float4(left + pre[0], left + pre[1], left + pre[2], left + pre[3]));
+                sts4(gt + 4 * GT_H, make_float4(hv[0], hv[1], hv[2], hv[3]));
+                sts4(gt + 4 * GT_W, make_float4(hv[0] * f, hv[1] * f, hv[2] * f, hv[3] * f));
+                if (lane == 0) sts4(sums(buf, s), make_float4(R[0], R[1], R[2], R[3]));
             }
             warp_arrive(B_PF + buf);
         }
