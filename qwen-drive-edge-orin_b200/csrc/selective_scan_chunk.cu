@@ -124,7 +124,13 @@ struct ChunkParams {
     int seg_tokens;    // tokens per segment (a multiple of 128), 0: one segment per sequence
 };
 
-__device__ __noinline__ void scan_wait_failed(unsigned int* status) { atomicOr(status, 1u | (1u << 16)); }
+// The rest of a wait whose first test failed, out of line (the kernel has some thirty waits and is
+// sensitive to instruction fetch): false, and bits 0 and 16 of the status word, when it ran out.
+__device__ __noinline__ bool scan_wait(uint32_t bar, uint32_t parity, unsigned int* status) {
+    if (ptx::mbar_wait_compact(bar, parity, WAIT_ITERS)) return true;
+    atomicOr(status, 1u | (1u << 16));
+    return false;
+}
 
 __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3) {
     asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
@@ -340,10 +346,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
     // whatever is there (every access stays in its buffer), issuing threads stop.
     bool dead = false;
     auto wait = [&](int b, uint32_t parity) {
-        if (!dead && !ptx::mbar_wait_compact(bar(b), parity & 1u, WAIT_ITERS)) {
-            dead = true;
-            scan_wait_failed(p.status);
-        }
+        if (!dead && !ptx::mbar_test_wait(bar(b), parity & 1u)) dead = !scan_wait(bar(b), parity & 1u, p.status);
     };
     auto warp_wait = [&](int b, uint32_t parity) {
         wait(b, parity);
@@ -411,11 +414,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
     // The rows behind the sequence in its last tiles belong to others and may hold anything: zeros, as
     // their products would otherwise reach valid rows as 0 x NaN. Rows [lo, hi) of a panel, by one warpgroup.
     auto zero_rows = [&](uint32_t panel, int lo, int hi) {
+#pragma unroll 1
         for (int e = tid & 127; e < (hi - lo) * 8; e += 128) st_shared_v4(row_at(panel, lo + (e >> 3)) ^ ((e & 7) << 4), 0, 0, 0, 0);
         ptx::fence_proxy_async_smem();
     };
     auto zero_x = [&](int k, int valid) {  // this warpgroup's tokens, both slots
         if (valid >= PIECE * (wg + 1)) return;
+#pragma unroll 1
         for (int s = 0; s < 2; ++s) zero_rows(sb + OFF_X + (2 * (k & 1) + s) * PANEL, max(valid, PIECE * wg), PIECE * (wg + 1));
     };
     // Both slots of one head (a head of more than 64 channels, or an odd slot run twice): one M for both.
@@ -677,6 +682,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
     } else if (warp == 16 || warp == 19) {
         // ================= MMA issue (one thread of each warp) =================
         if (elect_one()) {
+            // (inline waits: behind a call the compiler no longer keeps the descriptors uniform)
+            auto wait = [&](int b, uint32_t parity) {
+                if (!dead && !ptx::mbar_wait_compact(bar(b), parity & 1u, WAIT_ITERS)) {
+                    dead = true;
+                    atomicOr(p.status, 1u | (1u << 16));
+                }
+            };
             constexpr uint32_t ID_G = ptx::idesc_bf16(128, 128, 0, 0, 0);      // C B^T, C S^T
             constexpr uint32_t ID_INTRA = ptx::idesc_bf16(128, 64, 0, 1, 0);   // M X         (A in TMEM, B MN-major)
             constexpr uint32_t ID_TWIN = ptx::idesc_bf16(128, 128, 0, 1, 0);   // M X of both slots
@@ -770,6 +782,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 if (dead || k >= nc) return;
                 ++nb;
                 ptx::mbar_arrive_expect_tx(bar(B_BF + (k & 1)), npanel * PANEL);
+#pragma unroll 1
                 for (int c = 0; c < npanel; ++c)
                     ptx::tma_load_4d(sb + b_off(k) + c * PANEL, &p.tm_b, bar(B_BF + (k & 1)), 64 * c, g, row0 + CH * k, 0);
             };
@@ -777,6 +790,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 if (dead || k >= nc) return;
                 ++ncl;
                 ptx::mbar_arrive_expect_tx(bar(B_CF), npanel * PANEL);
+#pragma unroll 1
                 for (int c = 0; c < npanel; ++c) ptx::tma_load_4d(sb + OFF_C + c * PANEL, &p.tm_c, bar(B_CF), 64 * c, g, row0 + CH * k, 0);
             };
             auto load_x = [&](int k) {
@@ -787,33 +801,33 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 ptx::tma_load_4d(sb + OFF_X + 2 * buf * PANEL, &p.tm_x, bar(B_XF + buf), t0, h0, row0 + CH * k, 0);
                 ptx::tma_load_4d(sb + OFF_X + (2 * buf + 1) * PANEL, &p.tm_x, bar(B_XF + buf), t1, h1, row0 + CH * k, 0);
             };
-            load_x(0);
-            load_b(0);
-            if (!kState) load_c(0);
-            load_x(1);
-            load_b(1);
-            for (int k = 0; k < nc && !dead; ++k) {
+#pragma unroll 1
+            for (int k = -2; k < nc && !dead; ++k) {  // (one copy of each load: the first two rounds only fill the buffers)
+                const int buf = k & 1;
                 if constexpr (kState) {
-                    wait(B_XE + (k & 1), (uint32_t)k >> 1);
+                    if (k >= 0) wait(B_XE + buf, (uint32_t)k >> 1);
                     load_x(k + 2);
-                    wait(B_BE + (k & 1), (uint32_t)k >> 1);
+                    if (k >= 0) wait(B_BE + buf, (uint32_t)k >> 1);
                     load_b(k + 2);
                 } else {
-                    if (k + 1 < nc)  // the next C tile on its way to L2 while its buffer is in use
+                    if (k >= 0 && k + 1 < nc)  // the next C tile on its way to L2 while its buffer is in use
+#pragma unroll 1
                         for (int c = 0; c < npanel; ++c) ptx::tma_prefetch_4d(&p.tm_c, 64 * c, g, row0 + CH * (k + 1), 0);
-                    wait(B_ID, k);  // (behind it, by the same thread, G of this chunk: B is free with the state product)
-                    load_c(k + 1);
-                    wait(B_BE + (k & 1), (uint32_t)k >> 1);
+                    if (k >= 0) wait(B_ID, k);  // (behind it, by the same thread, G of this chunk: B is free with the state product)
+                    if (k >= -1) load_c(k + 1);
+                    if (k >= 0) wait(B_BE + buf, (uint32_t)k >> 1);
                     load_b(k + 2);
-                    if (len - CH * k >= CH) {  // a full tile: out by TMA (the warps store a partial one themselves)
-                        const int buf = k & 1, row = row0 + CH * k;
-                        wait(B_YS + buf, (uint32_t)k >> 1);
-                        if (!dead) tma_store_4d(&p.tm_y, sb + OFF_X + 2 * buf * PANEL, t0, h0, row, 0);
-                        wait(B_YS + 2 + buf, (uint32_t)k >> 1);
-                        if (!dead && second) tma_store_4d(&p.tm_y, sb + OFF_X + (2 * buf + 1) * PANEL, t1, h1, row, 0);
+                    if (k >= 0 && len - CH * k >= CH) {  // a full tile: out by TMA (the warps store a partial one themselves)
+                        const int row = row0 + CH * k;
+#pragma unroll 1
+                        for (int s = 0; s < 2; ++s) {
+                            wait(B_YS + 2 * s + buf, (uint32_t)k >> 1);
+                            if (!dead && (s == 0 || second))
+                                tma_store_4d(&p.tm_y, sb + OFF_X + (2 * buf + s) * PANEL, s ? t1 : t0, s ? h1 : h0, row, 0);
+                        }
                         ptx::bulk_wait_read_all();
-                        load_x(k + 2);
                     }
+                    load_x(k + 2);  // (chunk k + 2 exists: chunk k was full)
                 }
             }
             // nothing in flight when the CTA leaves
@@ -831,75 +845,71 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
     } else if (warp == 18) {
         // ================= gates of both slots =================
         float A2[2], bias[2], next[2][4];
-        const int row0 = seg[SEG_ROW], hd[2] = {slot_head(0), slot_head(1)};
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            A2[s] = a.A[hd[s]] * LOG2E;
-            bias[s] = a.dt_bias ? a.dt_bias[hd[s]] : 0.f;
-        }
-        auto load = [&](int k) {  // clamped to the segment's rows
-            const int last = len - 1 - CH * k;
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) next[s][i] = scan_dt(a, (int64_t)row0 + CH * k + min(4 * lane + i, last), hd[s]);
-        };
-        if (nc > 0) load(0);
-        for (int k = 0; k < nc; ++k) {
-            const int buf = k & 1, valid = len - CH * k;
-            float d[2][4];
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
+        const int h0 = slot_head(0), h1 = slot_head(1);
+        const int64_t row0 = seg[SEG_ROW];
+        A2[0] = a.A[h0] * LOG2E, A2[1] = a.A[h1] * LOG2E;
+        bias[0] = a.dt_bias ? a.dt_bias[h0] : 0.f, bias[1] = a.dt_bias ? a.dt_bias[h1] : 0.f;
+#pragma unroll 1
+        for (int k = -1; k < nc; ++k) {
+            float ahead[2][4];  // the next chunk's steps, four tokens a lane, clamped to the segment's rows
+            if (k + 1 < nc) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float v = next[s][i] + bias[s];
-                    if (a.softplus) v = softplus_series(v);
-                    d[s][i] = 4 * lane + i < valid ? v : 0.f;
+                    const int64_t at = (row0 + min(CH * (k + 1) + 4 * lane + i, len - 1)) * a.dts;
+                    ahead[0][i] = a.dt_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.dt)[at + h0]) : static_cast<const float*>(a.dt)[at + h0];
+                    ahead[1][i] = a.dt_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.dt)[at + h1]) : static_cast<const float*>(a.dt)[at + h1];
                 }
-            if (k + 1 < nc) load(k + 1);
-            if (k >= 2) warp_wait(B_PE + buf, ((uint32_t)k >> 1) - 1);
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-                sts4(gates(buf, s) + 4 * (GT_D + 4 * lane), make_float4(d[s][0], d[s][1], d[s][2], d[s][3]));
-#pragma unroll 1
-            for (int s = 0; s < 2; ++s) {
-                const uint32_t gt = gates(buf, s) + 16 * lane;
-                const float4 d4 = lds4(gt + 4 * GT_D);
-                const float A2s = s ? A2[1] : A2[0];
-                // log2 decays; the clamp keeps sums of 128 finite, and 2^-1e30 is zero as well
-                float pre[4], suf[4];
-                const float t0 = fmaxf(d4.x * A2s, -1e30f), t1 = fmaxf(d4.y * A2s, -1e30f), t2 = fmaxf(d4.z * A2s, -1e30f),
-                            t3 = fmaxf(d4.w * A2s, -1e30f);
-                pre[0] = t0, pre[1] = t0 + t1, pre[2] = pre[1] + t2, pre[3] = pre[2] + t3;
-                suf[3] = 0.f, suf[2] = t3, suf[1] = t3 + t2, suf[0] = suf[1] + t1;
-                // sums over the 8 lanes of a 32-token block, from the left and, for the accuracy of the
-                // short distances, from the right
-                float inc = pre[3], dec = pre[3];
-#pragma unroll
-                for (int off = 1; off < 8; off <<= 1) {
-                    const float u = __shfl_up_sync(0xffffffffu, inc, off, 8), v = __shfl_down_sync(0xffffffffu, dec, off, 8);
-                    if ((lane & 7) >= off) inc += u;
-                    if ((lane & 7) + off < 8) dec += v;
-                }
-                float left = __shfl_up_sync(0xffffffffu, inc, 1, 8), right = __shfl_down_sync(0xffffffffu, dec, 1, 8);
-                if ((lane & 7) == 0) left = 0.f;
-                if ((lane & 7) == 7) right = 0.f;
-                float R[4];
-#pragma unroll
-                for (int b = 0; b < 4; ++b) R[b] = __shfl_sync(0xffffffffu, inc, 8 * b + 7);
-                float behind = 0.f;
-#pragma unroll
-                for (int b = 3; b > 0; --b)
-                    if (b > (lane >> 3)) behind += R[b];
-                const float f = ex2f(behind);
-                const float hv[4] = {ex2f(right + suf[0]) * d4.x, ex2f(right + suf[1]) * d4.y, ex2f(right + suf[2]) * d4.z,
-                                     ex2f(right + suf[3]) * d4.w};
-                sts4(gt + 4 * GT_C, make_float4(left + pre[0], left + pre[1], left + pre[2], left + pre[3]));
-                sts4(gt + 4 * GT_H, make_float4(hv[0], hv[1], hv[2], hv[3]));
-                sts4(gt + 4 * GT_W, make_float4(hv[0] * f, hv[1] * f, hv[2] * f, hv[3] * f));
-                if (lane == 0) sts4(sums(buf, s), make_float4(R[0], R[1], R[2], R[3]));
             }
-            warp_arrive(B_PF + buf);
+            const int buf = k & 1, valid = len - CH * k;
+            if (k >= 2) warp_wait(B_PE + buf, ((uint32_t)k >> 1) - 1);
+#pragma unroll 1
+            for (int s = 0; k >= 0 && s < 2; ++s) {
+            float d[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                d[i] = (s ? next[1][i] : next[0][i]) + (s ? bias[1] : bias[0]);
+                if (a.softplus) d[i] = softplus_series(d[i]);
+                d[i] = 4 * lane + i < valid ? d[i] : 0.f;
+            }
+            const uint32_t gt = gates(buf, s) + 16 * lane;
+            const float A2s = s ? A2[1] : A2[0];
+            // log2 decays; the clamp keeps sums of 128 finite, and 2^-1e30 is zero as well
+            float t[4], pre[4], suf[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[i] = fmaxf(d[i] * A2s, -1e30f);
+            pre[0] = t[0], pre[1] = t[0] + t[1], pre[2] = pre[1] + t[2], pre[3] = pre[2] + t[3];
+            suf[3] = 0.f, suf[2] = t[3], suf[1] = t[3] + t[2], suf[0] = suf[1] + t[1];
+            // sums over the 8 lanes of a 32-token block, from the left and, for the accuracy of the
+            // short distances, from the right
+            float inc = pre[3], dec = pre[3];
+#pragma unroll
+            for (int off = 1; off < 8; off <<= 1) {
+                const float u = __shfl_up_sync(0xffffffffu, inc, off, 8), v = __shfl_down_sync(0xffffffffu, dec, off, 8);
+                if ((lane & 7) >= off) inc += u;
+                if ((lane & 7) + off < 8) dec += v;
+            }
+            float left = __shfl_up_sync(0xffffffffu, inc, 1, 8), right = __shfl_down_sync(0xffffffffu, dec, 1, 8);
+            if ((lane & 7) == 0) left = 0.f;
+            if ((lane & 7) == 7) right = 0.f;
+            float R[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) R[b] = __shfl_sync(0xffffffffu, inc, 8 * b + 7);
+            float behind = 0.f;
+#pragma unroll
+            for (int b = 3; b > 0; --b)
+                if (b > (lane >> 3)) behind += R[b];
+            const float f = ex2f(behind);
+            const float hv[4] = {ex2f(right + suf[0]) * d[0], ex2f(right + suf[1]) * d[1], ex2f(right + suf[2]) * d[2],
+                                 ex2f(right + suf[3]) * d[3]};
+            sts4(gt + 4 * GT_D, make_float4(d[0], d[1], d[2], d[3]));
+            sts4(gt + 4 * GT_C, make_float4(left + pre[0], left + pre[1], left + pre[2], left + pre[3]));
+            sts4(gt + 4 * GT_H, make_float4(hv[0], hv[1], hv[2], hv[3]));
+            sts4(gt + 4 * GT_W, make_float4(hv[0] * f, hv[1] * f, hv[2] * f, hv[3] * f));
+            if (lane == 0) sts4(sums(buf, s), make_float4(R[0], R[1], R[2], R[3]));
+            }
+            if (k >= 0) warp_arrive(B_PF + buf);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) next[0][i] = ahead[0][i], next[1][i] = ahead[1][i];
         }
     }
     ptx::tc_fence_before();
