@@ -239,7 +239,9 @@ __device__ __forceinline__ uint32_t top_halves(float a, float b) {  // bf16 pair
 }
 __device__ __forceinline__ float head(float a) { return __uint_as_float(__float_as_uint(a) & 0xFFFF0000u); }
 
-// kState: the state pass of a segmented call: every segment but a sequence's last from a zero state;
+// kState: the state pass of a segmented call: every segment but a sequence's last from a zero state. With
+// weights that decay to the segment's end (chunks in reverse order, the later chunks' decay carried along)
+// the state is one long product: no decay of the state, no chain between chunks, four pieces in flight;
 // its final state and log decay go to part / part_log, no output.
 template <bool kState>
 __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __grid_constant__ ChunkParams p) {
@@ -261,6 +263,19 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
             seq = sid / count;
             first = seq * count;
             j = sid - first;
+        } else if (p.seg_tokens == 0 && a.cu != nullptr && a.N <= 32) {  // packed: the longest sequences first
+            int64_t b = 0, e = -1;
+            if (lane < a.N) seq_range(a.cu, lane, a.T, b, e);
+            const int n = (int)(e - b);
+            int rank = 0;
+#pragma unroll 1
+            for (int o = 0; o < 32; ++o) {
+                const int other = __shfl_sync(0xffffffffu, n, o);
+                rank += other > n || (other == n && o < lane);
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, lane < a.N && rank == sid);
+            seq = hit ? __ffs(hit) - 1 : a.N;
+            first = 0;
         } else if (p.seg_tokens > 0) {  // packed: segments in the order of the sequences
             int base = 0;
             seq = a.N;
@@ -352,6 +367,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
         wait(b, parity);
         __syncwarp();
     };
+    // first token row of chunk k of the walk
+    auto chunk_row = [&](int row0, int k) { return row0 + CH * (kState ? nc - 1 - k : k); };
     auto b_off = [](int k) { return OFF_B + (uint32_t)(k & 1) * 2 * PANEL; };
     // Warps 0-15: one warp of a warpgroup polls (`f` waits), the others sleep in a named barrier until it has
     // seen all: twenty polling warps took a third of the issue slots.
@@ -376,7 +393,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
         uint32_t gt = gates(k & 1, s) + 4 * (GT_W + PIECE * wg);
         // token t of the piece: rows of 128 bytes whose 16-byte chunks are swizzled by t & 7
         uint32_t at = sb + OFF_X + (2 * (k & 1) + s) * PANEL + PIECE * wg * 128 + ((p >> 3) << 4) + ((p & 7) << 1);
-        uint32_t to = tl + TM_X + TM_XP * (wg & 1);
+        uint32_t to = tl + (kState ? TM_G + TM_XP * wg : TM_X + TM_XP * (wg & 1));
         ptx::tc_fence_after();
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
@@ -433,9 +450,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
         const bool second_half = warp >= 8;
         const int cols = wg & 1;  // y: slot; state: 64-column panel
         const uint32_t tm_s = tl + TM_S + 64 * cols, tm_y = tl + TM_Y + 64 * cols;
-        float D = 0.f, log_decay = 0.f;
+        float D = 0.f;
         if (!kState && second_half && a.D != nullptr) D = a.D[slot_head(cols)];
-        if (second_half && !idle) {  // entry state: the initial state carried through the earlier segments
+        if (!kState && second_half && !idle) {  // entry state: the initial state carried through the earlier segments
             const int s = quarter >> 1, ch = slot_tile(s) + (row & 63), seg_first = seg[SEG_FIRST], seg_j = seg[SEG_J];
             const size_t sbase = (((size_t)seg[SEG_SEQ] * a.H + slot_head(s)) * a.P + ch) * a.NS + 64 * cols;
             const bool inside = !kState && a.s0 != nullptr && ch < a.P;
@@ -515,6 +532,26 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 }
             }
         };
+        if constexpr (kState) {  // (segments of the state pass are whole chunks)
+#pragma unroll 1
+            for (int k = 0; k < nc; ++k) {
+                const int buf = k & 1;
+                team_wait([&] {
+                    wait(B_PF + buf, (uint32_t)k >> 1);
+                    wait(B_XF + buf, (uint32_t)k >> 1);
+                    if (k > 0) wait(B_RE + wg, k - 1);
+                });
+                piece(k);
+                if (lane == 0) {
+                    ptx::mbar_arrive(bar(B_PE + buf));
+                    ptx::mbar_arrive(bar(B_XE + buf));
+                }
+            }
+            if (second_half && nc > 0) {
+                team_wait([&] { wait(B_SD, 0); });
+                ptx::tc_fence_after();
+            }
+        } else {
 #pragma unroll 1
         for (int k = second_half ? 0 : -1; k < nc + (second_half ? 1 : 0); ++k) {
             const int buf = k & 1;
@@ -525,13 +562,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                     team_wait([&] {
                         wait(B_PF + buf, (uint32_t)k >> 1);
                         if (k > 0) wait(B_SD, k - 1);
-                        if (!kState && k > 0) wait(B_ID, k - 1);  // the last operand has been read
+                        if (k > 0) wait(B_ID, k - 1);  // the last operand has been read
                     });
                     ptx::tc_fence_after();
                     if (cols < npanel) {
                         const float4 R = lds4(sums(buf, quarter >> 1));
                         const float total = (R.x + R.y) + (R.z + R.w);
-                        log_decay += total;
                         const float decay = ex2f(total);
                         const uint64_t dd = f2_pack(decay, decay);
 #pragma unroll 1
@@ -539,7 +575,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                             uint32_t v[32];
                             tmem_ld32u(tm_s + 32 * hf, v);
                             ptx::tmem_wait_ld();
-                            if constexpr (!kState) {
+                            {
                                 uint32_t at = row_at(sb + OFF_S + cols * PANEL, row);
                                 keep_local(at);
 #pragma unroll
@@ -567,10 +603,10 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                     team_wait([&] { wait(B_SD, nc - 1); });
                     ptx::tc_fence_after();
                 }
-                if (!kState && k > 0) output(k - 1);
+                if (k > 0) output(k - 1);
             } else if (k >= 0) {
                 const int q = quarter;
-                if constexpr (!kState) {
+                {
                     team_wait([&] { wait(B_GF, k); });
                     ptx::tc_fence_after();
                     // M_ij = G_ij h_j 2^{c_i + (sum of a over the blocks between)}: blocks 0, 2 of this warp's
@@ -634,10 +670,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                     ptx::tc_fence_before();
                     warp_arrive(B_MR);
                 }
-                if (lane == 0) {
-                    ptx::mbar_arrive(bar(B_PE + buf));
-                    if (kState) ptx::mbar_arrive(bar(B_XE + buf));
-                }
+                if (lane == 0) ptx::mbar_arrive(bar(B_PE + buf));
             }
             const int kp = second_half ? k : k + 1;
             if (kp < nc) {
@@ -653,17 +686,14 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                     ptx::named_sync(1 + wg, 128);
                 }
                 piece(kp);
-                if (second_half && lane == 0) {
-                    ptx::mbar_arrive(bar(B_PE + buf));
-                    if (kState) ptx::mbar_arrive(bar(B_XE + buf));
-                }
+                if (second_half && lane == 0) ptx::mbar_arrive(bar(B_PE + buf));
             }
+        }
         }
         if (second_half && !idle && (kState || seg[SEG_J] == seg[SEG_COUNT] - 1)) {
             const int s = quarter >> 1, ch = slot_tile(s) + (row & 63);
             const size_t sbase = (((size_t)seg[SEG_SEQ] * a.H + slot_head(s)) * a.P + ch) * a.NS + 64 * cols;
             const bool inside = ch < a.P && (s == 0 || seg[SEG_SECOND]);
-            if (kState && cols == 0 && (row & 63) == 0) p.part_log[2 * (size_t)blockIdx.x + s] = log_decay;
 #pragma unroll 1
             for (int q4 = 0; q4 < 4; ++q4) {
                 float v[16];
@@ -700,7 +730,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 const uint32_t id_state = ptx::idesc_bf16(128, 16 * ks, 0, 1, 0);  // X'^T B  (A in TMEM, B MN-major)
                 for (int k = 0; k < nc; ++k) {
                     wait(B_BF + (k & 1), (uint32_t)k >> 1);
-                    wait(B_SC, k);
+                    if (!kState) wait(B_SC, k);
 #pragma unroll 1
                     for (int i = 0; i < PIECES; ++i) {
                         wait(B_RF + i, k);
@@ -710,12 +740,14 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                         for (int st = 0; st < PIECE / 16; ++st)
 #pragma unroll
                             for (int term = 0; term < 3; ++term)
-                                ptx::mma_bf16_ts(tmem + TM_S, tmem + TM_X + TM_XP * (i & 1) + 16 * term + 8 * st,
-                                                 desc(dpanel, b_off(k) + (uint32_t)(PIECE * i + 16 * st) * 128u), id_state, 1);
+                                ptx::mma_bf16_ts(tmem + TM_S,
+                                                 tmem + (kState ? TM_G + TM_XP * i : TM_X + TM_XP * (i & 1)) + 16 * term + 8 * st,
+                                                 desc(dpanel, b_off(k) + (uint32_t)(PIECE * i + 16 * st) * 128u), id_state,
+                                                 !kState || k + i + st + term > 0);
                         ptx::mma_commit(bar(B_RE + i));
                     }
                     if (dead) break;
-                    ptx::mma_commit(bar(B_SD));
+                    if (!kState || k == nc - 1) ptx::mma_commit(bar(B_SD));
                     ptx::mma_commit(bar(B_BE + (k & 1)));
                 }
             } else if (!kState) {
@@ -784,7 +816,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 ptx::mbar_arrive_expect_tx(bar(B_BF + (k & 1)), npanel * PANEL);
 #pragma unroll 1
                 for (int c = 0; c < npanel; ++c)
-                    ptx::tma_load_4d(sb + b_off(k) + c * PANEL, &p.tm_b, bar(B_BF + (k & 1)), 64 * c, g, row0 + CH * k, 0);
+                    ptx::tma_load_4d(sb + b_off(k) + c * PANEL, &p.tm_b, bar(B_BF + (k & 1)), 64 * c, g, chunk_row(row0, k), 0);
             };
             auto load_c = [&](int k) {
                 if (dead || k >= nc) return;
@@ -798,8 +830,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 ++nx;
                 const int buf = k & 1;
                 ptx::mbar_arrive_expect_tx(bar(B_XF + buf), 2 * PANEL);
-                ptx::tma_load_4d(sb + OFF_X + 2 * buf * PANEL, &p.tm_x, bar(B_XF + buf), t0, h0, row0 + CH * k, 0);
-                ptx::tma_load_4d(sb + OFF_X + (2 * buf + 1) * PANEL, &p.tm_x, bar(B_XF + buf), t1, h1, row0 + CH * k, 0);
+                ptx::tma_load_4d(sb + OFF_X + 2 * buf * PANEL, &p.tm_x, bar(B_XF + buf), t0, h0, chunk_row(row0, k), 0);
+                ptx::tma_load_4d(sb + OFF_X + (2 * buf + 1) * PANEL, &p.tm_x, bar(B_XF + buf), t1, h1, chunk_row(row0, k), 0);
             };
 #pragma unroll 1
             for (int k = -2; k < nc && !dead; ++k) {  // (one copy of each load: the first two rounds only fill the buffers)
@@ -844,7 +876,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
         __syncwarp();
     } else if (warp == 18) {
         // ================= gates of both slots =================
-        float A2[2], bias[2], next[2][4];
+        float A2[2], bias[2], next[2][4], later[2] = {0.f, 0.f};  // (later: log2 decay of the chunks behind, state pass)
         const int h0 = slot_head(0), h1 = slot_head(1);
         const int64_t row0 = seg[SEG_ROW];
         A2[0] = a.A[h0] * LOG2E, A2[1] = a.A[h1] * LOG2E;
@@ -855,12 +887,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
             if (k + 1 < nc) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int64_t at = (row0 + min(CH * (k + 1) + 4 * lane + i, len - 1)) * a.dts;
+                    const int64_t at = (row0 + min(chunk_row(0, k + 1) + 4 * lane + i, len - 1)) * a.dts;
                     ahead[0][i] = a.dt_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.dt)[at + h0]) : static_cast<const float*>(a.dt)[at + h0];
                     ahead[1][i] = a.dt_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.dt)[at + h1]) : static_cast<const float*>(a.dt)[at + h1];
                 }
             }
-            const int buf = k & 1, valid = len - CH * k;
+            const int buf = k & 1, valid = kState ? CH : len - CH * k;
             if (k >= 2) warp_wait(B_PE + buf, ((uint32_t)k >> 1) - 1);
 #pragma unroll 1
             for (int s = 0; k >= 0 && s < 2; ++s) {
@@ -898,6 +930,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
 #pragma unroll
             for (int b = 3; b > 0; --b)
                 if (b > (lane >> 3)) behind += R[b];
+            if (kState) {
+                behind += s ? later[1] : later[0];
+                const float total = (R[0] + R[1]) + (R[2] + R[3]);
+                if (s) later[1] += total;
+                else later[0] += total;
+            }
             const float f = ex2f(behind);
             const float hv[4] = {ex2f(right + suf[0]) * d[0], ex2f(right + suf[1]) * d[1], ex2f(right + suf[2]) * d[2],
                                  ex2f(right + suf[3]) * d[3]};
@@ -911,6 +949,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
 #pragma unroll
             for (int i = 0; i < 4; ++i) next[0][i] = ahead[0][i], next[1][i] = ahead[1][i];
         }
+        if (kState && !idle && lane == 0) p.part_log[2 * (size_t)blockIdx.x] = later[0], p.part_log[2 * (size_t)blockIdx.x + 1] = later[1];
     }
     ptx::tc_fence_before();
     __syncthreads();
@@ -974,16 +1013,21 @@ ChunkPlan plan_scan_chunks(int N, int T, bool packed, int H, int P, int G, int s
     pl.segments = N;
     const int64_t rows = packed ? T : (int64_t)N * T;
     const int64_t chunks = N > 0 ? (rows / N + CH - 1) / CH : 0;  // of the mean sequence
-    // Wave model. Measured on B200: an output pass takes about 1.8 us per chunk and pair and a state pass
-    // 1.1, a CTA's start and end about 5 us, the second launch 3 us. Segments pay where the
-    // (sequence, pair) units alone leave SMs idle.
-    auto waves = [&](int64_t ctas) { return (double)((ctas + sms - 1) / sms); };
-    double best = waves((int64_t)N * pl.units) * (1.8 * chunks + 5.0);
-    for (int64_t s = 2; s <= chunks && s <= 64 && (int64_t)N * pl.units * (s - 1) < sms; ++s) {
+    // Wave model. Measured on B200: an output pass takes about 4.1 us per chunk and pair and a state pass
+    // 1.1, a CTA's start and end about 4 us and the entry state 0.3 per earlier segment, the second launch 3 us.
+    // Segments pay where the (sequence, pair) units alone leave SMs idle. A packed batch's longest sequence
+    // is taken as twice the mean (the longest ones start first).
+    const int64_t ctas = (int64_t)N * pl.units;
+    auto waves = [&](int64_t n) { return (double)((n + sms - 1) / sms); };
+    double best = waves(ctas) * (4.1 * chunks + 4.0);
+    if (packed && N > 1) {
+        const double spread = (double)ctas * (4.1 * chunks + 4.0) / sms + 4.1 * chunks / 2, longest = 2 * 4.1 * chunks + 4.0;
+        best = spread > longest ? spread : longest;
+    }
+    for (int64_t s = 2; s <= chunks && s <= 64 && ctas * (s - 1) < 4 * sms; ++s) {
         const int64_t per = (chunks + s - 1) / s, cut = (chunks + per - 1) / per;
         if (cut < 2) continue;
-        const double t = waves((int64_t)N * pl.units * cut) * (1.8 * per + 5.0 + 0.4 * cut) +
-                         waves((int64_t)N * pl.units * (cut - 1)) * (1.1 * per + 5.0) + 3.0;
+        const double t = waves(ctas * cut) * (4.1 * per + 4.0 + 0.15 * cut) + waves(ctas * (cut - 1)) * (1.1 * per + 4.0) + 3.0;
         if (t < best) {
             best = t;
             pl.seg_tokens = (int)(per * CH);
