@@ -25,7 +25,9 @@
 //
 // Decays are kept as base-2 logarithms, relative to 32-token blocks: e^{c_i - c_j} is a row factor times
 // a column factor, one exponential per row and block. Across blocks both are at most 1; inside a block
-// the row factor undoes the column factor beyond the row, which fp32 holds for decays down to 2^-100.
+// the row factor undoes the column factor beyond the row, which fp32 holds for decays down to 2^-100
+// (below: an exponential per element). (A third way was tried and left out: the row factors taken out of
+// M and applied to the finished row where a chunk decays by less than 2^64; no faster.)
 //
 // Bound: shared memory, which feeds the MMAs' operands besides everything else (128 bytes a cycle and SM:
 // an MMA of 128 x 128 x 16 with both operands there takes all of it). So the two operands that the warps
@@ -69,7 +71,7 @@ constexpr uint32_t MISC_SUMS = 0;                    // block sums [2 buffers][2
 constexpr uint32_t MISC_BAR = 64;
 constexpr uint32_t MISC_TMEM = 344;
 constexpr uint32_t MISC_SEG = 348;                   // the CTA's segment and slots:
-enum { SEG_SEQ, SEG_J, SEG_COUNT, SEG_FIRST, SEG_ROW, SEG_LEN, SEG_HEAD, SEG_TILE = SEG_HEAD + 2, SEG_SECOND = SEG_TILE + 2,
+enum { SEG_SEQ, SEG_J, SEG_COUNT, SEG_ROW, SEG_LEN, SEG_HEAD, SEG_TILE = SEG_HEAD + 2, SEG_SECOND = SEG_TILE + 2,
        SEG_GROUP, SEG_WORDS };
 constexpr uint32_t MISC_BYTES = 448;
 static_assert(MISC_SEG + 4 * SEG_WORDS <= MISC_BYTES, "segment words overflow");
@@ -239,6 +241,58 @@ __device__ __forceinline__ uint32_t top_halves(float a, float b) {  // bf16 pair
 }
 __device__ __forceinline__ float head(float a) { return __uint_as_float(__float_as_uint(a) & 0xFFFF0000u); }
 
+// Segment sid of the call: sequence (a.N: there is none), segment j of `count` in it. One warp.
+__device__ __forceinline__ void find_segment(const ScanArgs& a, int seg_tokens, int sid, int lane, int& seq, int& j, int& count) {
+    int first = sid;
+    seq = sid, j = 0, count = 1;
+    if (seg_tokens > 0 && a.cu == nullptr) {
+        count = max(1, (a.T + seg_tokens - 1) / seg_tokens);
+        seq = sid / count;
+        first = seq * count;
+        j = sid - first;
+    } else if (seg_tokens == 0 && a.cu != nullptr && a.N <= 32) {  // packed: the longest sequences first
+        int64_t b = 0, e = -1;
+        if (lane < a.N) seq_range(a.cu, lane, a.T, b, e);
+        const int n = (int)(e - b);
+        int rank = 0;
+#pragma unroll 1
+        for (int o = 0; o < 32; ++o) {
+            const int other = __shfl_sync(0xffffffffu, n, o);
+            rank += other > n || (other == n && o < lane);
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, lane < a.N && rank == sid);
+        seq = hit ? __ffs(hit) - 1 : a.N;
+        first = 0;
+    } else if (seg_tokens > 0) {  // packed: segments in the order of the sequences
+        int base = 0;
+        seq = a.N;
+        for (int s0 = 0; s0 < a.N; s0 += 32) {
+            int n = 0;
+            if (s0 + lane < a.N) {
+                int64_t b, e;
+                seq_range(a.cu, s0 + lane, a.T, b, e);
+                n = max(1, (int)((e - b + seg_tokens - 1) / seg_tokens));
+            }
+            int inc = n;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int t = __shfl_up_sync(0xffffffffu, inc, off);
+                if (lane >= off) inc += t;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, base + inc > sid);
+            if (hit) {
+                const int src = __ffs(hit) - 1;
+                seq = s0 + src;
+                count = __shfl_sync(0xffffffffu, n, src);
+                first = base + __shfl_sync(0xffffffffu, inc, src) - count;
+                j = sid - first;
+                break;
+            }
+            base += __shfl_sync(0xffffffffu, inc, 31);
+        }
+    }
+}
+
 // kState: the state pass of a segmented call: every segment but a sequence's last from a zero state. With
 // weights that decay to the segment's end (chunks in reverse order, the later chunks' decay carried along)
 // the state is one long product: no decay of the state, no chain between chunks, four pieces in flight;
@@ -257,53 +311,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
     // ---- this CTA's segment ----
     if (warp == 0) {
         const int unit = blockIdx.x % p.units, sid = blockIdx.x / p.units;
-        int seq = sid, j = 0, first = sid, count = 1;
-        if (p.seg_tokens > 0 && a.cu == nullptr) {
-            count = max(1, (a.T + p.seg_tokens - 1) / p.seg_tokens);
-            seq = sid / count;
-            first = seq * count;
-            j = sid - first;
-        } else if (p.seg_tokens == 0 && a.cu != nullptr && a.N <= 32) {  // packed: the longest sequences first
-            int64_t b = 0, e = -1;
-            if (lane < a.N) seq_range(a.cu, lane, a.T, b, e);
-            const int n = (int)(e - b);
-            int rank = 0;
-#pragma unroll 1
-            for (int o = 0; o < 32; ++o) {
-                const int other = __shfl_sync(0xffffffffu, n, o);
-                rank += other > n || (other == n && o < lane);
-            }
-            const unsigned hit = __ballot_sync(0xffffffffu, lane < a.N && rank == sid);
-            seq = hit ? __ffs(hit) - 1 : a.N;
-            first = 0;
-        } else if (p.seg_tokens > 0) {  // packed: segments in the order of the sequences
-            int base = 0;
-            seq = a.N;
-            for (int s0 = 0; s0 < a.N; s0 += 32) {
-                int n = 0;
-                if (s0 + lane < a.N) {
-                    int64_t b, e;
-                    seq_range(a.cu, s0 + lane, a.T, b, e);
-                    n = max(1, (int)((e - b + p.seg_tokens - 1) / p.seg_tokens));
-                }
-                int inc = n;
-#pragma unroll
-                for (int off = 1; off < 32; off <<= 1) {
-                    const int t = __shfl_up_sync(0xffffffffu, inc, off);
-                    if (lane >= off) inc += t;
-                }
-                const unsigned hit = __ballot_sync(0xffffffffu, base + inc > sid);
-                if (hit) {
-                    const int src = __ffs(hit) - 1;
-                    seq = s0 + src;
-                    count = __shfl_sync(0xffffffffu, n, src);
-                    first = base + __shfl_sync(0xffffffffu, inc, src) - count;
-                    j = sid - first;
-                    break;
-                }
-                base += __shfl_sync(0xffffffffu, inc, 31);
-            }
-        }
+        int seq, j, count;
+        find_segment(a, p.seg_tokens, sid, lane, seq, j, count);
         if (lane == 0) {
             int64_t b = 0, e = 0;
             if (seq < a.N) seq_range(a.cu, seq, a.T, b, e);
@@ -312,7 +321,6 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
             seg[SEG_SEQ] = seq;
             seg[SEG_J] = j;
             seg[SEG_COUNT] = count;
-            seg[SEG_FIRST] = first;
             seg[SEG_ROW] = begin;
             seg[SEG_LEN] = (p.seg_tokens > 0) ? min(p.seg_tokens, (int)e - begin) : (int)(e - b);
             // slots: head and channel tile; an odd one out runs its slot twice and stores it once
@@ -452,8 +460,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
         const uint32_t tm_s = tl + TM_S + 64 * cols, tm_y = tl + TM_Y + 64 * cols;
         float D = 0.f;
         if (!kState && second_half && a.D != nullptr) D = a.D[slot_head(cols)];
-        if (!kState && second_half && !idle) {  // entry state: the initial state carried through the earlier segments
-            const int s = quarter >> 1, ch = slot_tile(s) + (row & 63), seg_first = seg[SEG_FIRST], seg_j = seg[SEG_J];
+        if (!kState && second_half && !idle) {  // entry state: the initial state, or the one that scan_entry_kernel left
+            const int s = quarter >> 1, ch = slot_tile(s) + (row & 63);
+            const bool later = seg[SEG_J] > 0;
             const size_t sbase = (((size_t)seg[SEG_SEQ] * a.H + slot_head(s)) * a.P + ch) * a.NS + 64 * cols;
             const bool inside = !kState && a.s0 != nullptr && ch < a.P;
 #pragma unroll 1
@@ -462,23 +471,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (inside && 64 * cols + 16 * q4 + 4 * c < a.NS) f = *reinterpret_cast<const float4*>(a.s0 + sbase + 16 * q4 + 4 * c);
+                    if (later) f = p.part[((size_t)blockIdx.x * 32 + 16 * cols + 4 * q4 + c) * CH + row];
+                    else if (inside && 64 * cols + 16 * q4 + 4 * c < a.NS) f = *reinterpret_cast<const float4*>(a.s0 + sbase + 16 * q4 + 4 * c);
                     v[4 * c] = f.x, v[4 * c + 1] = f.y, v[4 * c + 2] = f.z, v[4 * c + 3] = f.w;
-                }
-                if constexpr (!kState) {
-                    for (int e = seg_first; e < seg_first + seg_j; ++e) {
-                        const size_t at = (size_t)e * p.units + blockIdx.x % p.units;
-                        const float decay = ex2f(p.part_log[2 * at + s]);
-                        const float4* src = p.part + (at * 32 + 16 * cols + 4 * q4) * CH + row;
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const float4 f = src[c * CH];
-                            v[4 * c] = fmaf(decay, v[4 * c], f.x);
-                            v[4 * c + 1] = fmaf(decay, v[4 * c + 1], f.y);
-                            v[4 * c + 2] = fmaf(decay, v[4 * c + 2], f.z);
-                            v[4 * c + 3] = fmaf(decay, v[4 * c + 3], f.w);
-                        }
-                    }
                 }
                 uint32_t o[16];
 #pragma unroll
@@ -686,7 +681,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                     ptx::named_sync(1 + wg, 128);
                 }
                 piece(kp);
-                if (second_half && lane == 0) ptx::mbar_arrive(bar(B_PE + buf));
+                if (second_half) warp_arrive(B_PE + buf);
             }
         }
         }
@@ -941,8 +936,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                                  ex2f(right + suf[3]) * d[3]};
             sts4(gt + 4 * GT_D, make_float4(d[0], d[1], d[2], d[3]));
             sts4(gt + 4 * GT_C, make_float4(left + pre[0], left + pre[1], left + pre[2], left + pre[3]));
-            sts4(gt + 4 * GT_H, make_float4(hv[0], hv[1], hv[2], hv[3]));
             sts4(gt + 4 * GT_W, make_float4(hv[0] * f, hv[1] * f, hv[2] * f, hv[3] * f));
+            sts4(gt + 4 * GT_H, make_float4(hv[0], hv[1], hv[2], hv[3]));
             if (lane == 0) sts4(sums(buf, s), make_float4(R[0], R[1], R[2], R[3]));
             }
             if (k >= 0) warp_arrive(B_PF + buf);
@@ -955,6 +950,70 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
     __syncthreads();
     ptx::tc_fence_after();
     if (warp == 16) ptx::tmem_dealloc(tmem, 512);
+}
+
+// Entry states of the segments of each sequence, in place of their final states in `part`: from the
+// sequence's initial state, E_{j+1} = 2^{log_j} E_j + A_j. A thread owns a float4 of one (sequence, unit) and
+// walks the segments, eight of them loaded ahead.
+__global__ void __launch_bounds__(256) scan_entry_kernel(const __grid_constant__ ChunkParams p) {
+    __shared__ int found[2];
+    const ScanArgs& a = p.a;
+    const int unit = blockIdx.x % p.units, seq = blockIdx.x / p.units, lane = threadIdx.x & 31;
+    if (threadIdx.x < 32) {
+        int first = 0, count = 1;
+        if (a.cu == nullptr) {
+            count = max(1, (a.T + p.seg_tokens - 1) / p.seg_tokens);
+            first = seq * count;
+        } else {
+            for (int s0 = 0; s0 <= seq; s0 += 32) {  // segments of the sequences before
+                int n = 0;
+                if (s0 + lane <= seq) {
+                    int64_t b, e;
+                    seq_range(a.cu, s0 + lane, a.T, b, e);
+                    n = max(1, (int)((e - b + p.seg_tokens - 1) / p.seg_tokens));
+                }
+                const int own = __shfl_sync(0xffffffffu, n, (seq - s0) & 31);
+                if (s0 + 32 > seq) {
+                    count = own;
+                    if (lane == seq - s0) n = 0;
+                }
+                first += __reduce_add_sync(0xffffffffu, n);
+            }
+        }
+        if (lane == 0) found[0] = first, found[1] = count;
+    }
+    __syncthreads();
+    const int first = found[0], count = found[1];
+    if (count < 2) return;
+    const int g = unit / p.pairs, r_heads = a.H / a.G, slot0 = 2 * (unit - g * p.pairs);
+    const bool second = slot0 + 1 < r_heads * p.ptiles;
+    const int el = blockIdx.y * 256 + threadIdx.x, row = el & (CH - 1), n4 = el / CH, s = row >> 6;
+    const int slot = slot0 + (second ? s : 0), h = g * r_heads + slot / p.ptiles, ch = slot % p.ptiles * TILE + (row & 63);
+    float4 S = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (a.s0 != nullptr && ch < a.P && 4 * n4 < a.NS)
+        S = *reinterpret_cast<const float4*>(a.s0 + (((size_t)seq * a.H + h) * a.P + ch) * a.NS + 4 * n4);
+    const size_t step = (size_t)p.units * 32 * CH;
+    float4* at = p.part + ((size_t)first * p.units + unit) * 32 * CH + el;
+    const float* lg = p.part_log + 2 * ((size_t)first * p.units + unit) + s;
+    constexpr int AHEAD = 8;
+    for (int j0 = 0; j0 + 1 < count; j0 += AHEAD) {  // the state behind segment j is the entry state of j + 1
+        float4 A[AHEAD];
+        float l[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (j0 + i + 1 < count) A[i] = at[i * step], l[i] = lg[2 * (size_t)p.units * i];
+        // the last segment has no final state of its own here: its place only receives
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (j0 + i + 1 < count) {
+                if (j0 + i > 0) at[i * step] = S;
+                const float d = ex2f(l[i]);
+                S = make_float4(fmaf(d, S.x, A[i].x), fmaf(d, S.y, A[i].y), fmaf(d, S.z, A[i].z), fmaf(d, S.w, A[i].w));
+                if (j0 + i + 2 == count) at[(i + 1) * step] = S;
+            }
+        at += AHEAD * step;
+        lg += 2 * (size_t)p.units * AHEAD;
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -1061,6 +1120,8 @@ cudaError_t launch_scan_chunks(const ScanArgs& a, const ChunkPlan& pl, int64_t r
     if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
     if (pl.seg_tokens > 0) {
         scan_chunk_kernel<true><<<(unsigned)ctas, CHUNK_THREADS, CHUNK_SMEM, stream>>>(p);
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        scan_entry_kernel<<<dim3((unsigned)(a.N * pl.units), 32 * CH / 256), 256, 0, stream>>>(p);
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
     }
     scan_chunk_kernel<false><<<(unsigned)ctas, CHUNK_THREADS, CHUNK_SMEM, stream>>>(p);
