@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "gdn_ssm.h"
 #include "selective_scan.cuh"
 #include "ssm_common.cuh"
@@ -14,10 +16,12 @@ namespace ssm {
 constexpr int STEP_TOKENS = 6;
 
 static int sm_count() {
+    static std::atomic<int> known[64] = {};  // per device; threads that race here store the same value
     int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return 148;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if ((sms = known[dev].load(std::memory_order_relaxed)) > 0) return sms;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    known[dev].store(sms, std::memory_order_relaxed);
     return sms;
 }
 

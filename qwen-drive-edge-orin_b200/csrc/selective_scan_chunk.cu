@@ -243,13 +243,11 @@ __device__ __forceinline__ float head(float a) { return __uint_as_float(__float_
 
 // Segment sid of the call: sequence (a.N: there is none), segment j of `count` in it. One warp.
 __device__ __forceinline__ void find_segment(const ScanArgs& a, int seg_tokens, int sid, int lane, int& seq, int& j, int& count) {
-    int first = sid;
     seq = sid, j = 0, count = 1;
     if (seg_tokens > 0 && a.cu == nullptr) {
         count = max(1, (a.T + seg_tokens - 1) / seg_tokens);
         seq = sid / count;
-        first = seq * count;
-        j = sid - first;
+        j = sid - seq * count;
     } else if (seg_tokens == 0 && a.cu != nullptr && a.N <= 32) {  // packed: the longest sequences first
         int64_t b = 0, e = -1;
         if (lane < a.N) seq_range(a.cu, lane, a.T, b, e);
@@ -262,7 +260,6 @@ __device__ __forceinline__ void find_segment(const ScanArgs& a, int seg_tokens, 
         }
         const unsigned hit = __ballot_sync(0xffffffffu, lane < a.N && rank == sid);
         seq = hit ? __ffs(hit) - 1 : a.N;
-        first = 0;
     } else if (seg_tokens > 0) {  // packed: segments in the order of the sequences
         int base = 0;
         seq = a.N;
@@ -284,8 +281,7 @@ __device__ __forceinline__ void find_segment(const ScanArgs& a, int seg_tokens, 
                 const int src = __ffs(hit) - 1;
                 seq = s0 + src;
                 count = __shfl_sync(0xffffffffu, n, src);
-                first = base + __shfl_sync(0xffffffffu, inc, src) - count;
-                j = sid - first;
+                j = sid - (base + __shfl_sync(0xffffffffu, inc, src) - count);
                 break;
             }
             base += __shfl_sync(0xffffffffu, inc, 31);
@@ -308,6 +304,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
     const uint32_t bar0 = sb + OFF_MISC + MISC_BAR;
     auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
 
+    if (kState) ptx::grid_launch_dependents();
     // ---- this CTA's segment ----
     if (warp == 0) {
         const int unit = blockIdx.x % p.units, sid = blockIdx.x / p.units;
@@ -463,6 +460,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
         if (!kState && second_half && !idle) {  // entry state: the initial state, or the one that scan_entry_kernel left
             const int s = quarter >> 1, ch = slot_tile(s) + (row & 63);
             const bool later = seg[SEG_J] > 0;
+            if (later) ptx::grid_dependency_wait();
             const size_t sbase = (((size_t)seg[SEG_SEQ] * a.H + slot_head(s)) * a.P + ch) * a.NS + 64 * cols;
             const bool inside = !kState && a.s0 != nullptr && ch < a.P;
 #pragma unroll 1
@@ -946,6 +944,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
         }
         if (kState && !idle && lane == 0) p.part_log[2 * (size_t)blockIdx.x] = later[0], p.part_log[2 * (size_t)blockIdx.x + 1] = later[1];
     }
+    // an output pass ends after the passes before it, whether or not it needed them (the next launch in the
+    // stream waits for this one only)
+    if (!kState) ptx::grid_dependency_wait();
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
@@ -984,6 +985,8 @@ __global__ void __launch_bounds__(256) scan_entry_kernel(const __grid_constant__
     }
     __syncthreads();
     const int first = found[0], count = found[1];
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();  // the state pass's results
     if (count < 2) return;
     const int g = unit / p.pairs, r_heads = a.H / a.G, slot0 = 2 * (unit - g * p.pairs);
     const bool second = slot0 + 1 < r_heads * p.ptiles;
@@ -1118,14 +1121,30 @@ cudaError_t launch_scan_chunks(const ScanArgs& a, const ChunkPlan& pl, int64_t r
     p.seg_tokens = pl.seg_tokens;
     const int64_t ctas = pl.segments * pl.units;
     if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
-    if (pl.seg_tokens > 0) {
-        scan_chunk_kernel<true><<<(unsigned)ctas, CHUNK_THREADS, CHUNK_SMEM, stream>>>(p);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
-        scan_entry_kernel<<<dim3((unsigned)(a.N * pl.units), 32 * CH / 256), 256, 0, stream>>>(p);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    if (pl.seg_tokens == 0) {
+        scan_chunk_kernel<false><<<(unsigned)ctas, CHUNK_THREADS, CHUNK_SMEM, stream>>>(p);
+        return cudaGetLastError();
     }
-    scan_chunk_kernel<false><<<(unsigned)ctas, CHUNK_THREADS, CHUNK_SMEM, stream>>>(p);
-    return cudaGetLastError();
+    // State pass, entry states, output pass. The second and third are launched while the one before still
+    // runs (programmatic dependent launch) and wait for it where they read what it wrote; the first waits
+    // for the stream as usual, so the inputs are ready for all three.
+    scan_chunk_kernel<true><<<(unsigned)ctas, CHUNK_THREADS, CHUNK_SMEM, stream>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cfg.gridDim = dim3((unsigned)(a.N * pl.units), 32 * CH / 256, 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    if ((e = cudaLaunchKernelEx(&cfg, scan_entry_kernel, p)) != cudaSuccess) return e;
+    cfg.gridDim = dim3((unsigned)ctas, 1, 1);
+    cfg.blockDim = dim3(CHUNK_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = CHUNK_SMEM;
+    return cudaLaunchKernelEx(&cfg, scan_chunk_kernel<false>, p);
 }
 
 }  // namespace ssm

@@ -37,6 +37,11 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
+def _out(x):
+    """A contiguous tensor of x's shape, type and device."""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
 def _on_one_device(first, *others):
     """The index of the CUDA device that holds every tensor."""
     dev = first.get_device()
@@ -133,17 +138,22 @@ def _offsets(cu_seqlens, dev):
 # ---------------------------------------------------------------- causal convolution
 def _check_conv(x, w, bias, packed=False):
     dev = _on_one_device(x, w)
-    if x.dtype not in _DTYPES or w.dtype != x.dtype:
+    dtype = x.dtype
+    if dtype not in _DTYPES or w.dtype != dtype:
         raise ValueError("x and w must share dtype fp16, bf16 or fp32")
-    if x.dim() != 3 or w.dim() != 2 or w.shape[0] != x.shape[2]:
+    if x.dim() != 3 or w.dim() != 2:
         raise ValueError("bad shapes: x must be [B, T, C] and w [C, W]")
-    if not 2 <= w.shape[1] <= 4:
+    B, _, C = x.shape
+    rows, W = w.shape
+    if rows != C:
+        raise ValueError("bad shapes: x must be [B, T, C] and w [C, W]")
+    if not 2 <= W <= 4:
         raise ValueError("only 2 to 4 taps are supported")
-    if x.shape[2] < 1:
+    if C < 1:
         raise ValueError("x needs at least one channel")
-    if packed and x.shape[0] != 1:
+    if packed and B != 1:
         raise ValueError("varlen inputs are packed: B must be 1")
-    return dev, _vector(bias, x.shape[2], x.dtype, "bias", dev)
+    return dev, _vector(bias, C, dtype, "bias", dev)
 
 
 def _conv_prefill(x, w, bias, s0, silu, cu):
@@ -156,7 +166,7 @@ def _conv_prefill(x, w, bias, s0, silu, cu):
     s0 = _initial(s0, (n, W - 1, C), x.dtype, dev)
     x, stride = _rows(x, 2)
     w = w.contiguous()
-    y = x.new_empty((B, T, C))
+    y = _out(x)
     sf = x.new_empty((n, W - 1, C))
     _call(dev, "causal_conv_prefill", load_library().causal_conv_prefill, _p(x), stride, _p(w), _p(bias), _p(s0), _p(y),
           _p(sf), _p(cu), n, T, C, W, bool(silu), _DTYPES[x.dtype])
@@ -194,7 +204,7 @@ def causal_conv_decode(x, w, state, bias=None, silu: bool = True):
     _on_one_device(x, state)
     x, stride = _rows(x, 2)
     w = w.contiguous()
-    y = x.new_empty((B, T, C))
+    y = _out(x)
     _call(dev, "causal_conv_decode", load_library().causal_conv_decode, _p(x), stride, _p(w), _p(bias), _p(state), _p(y),
           B, T, C, W, bool(silu), _DTYPES[x.dtype])
     return y
@@ -232,7 +242,7 @@ def _scan_prefill(x, dt, A, B, C, D, dt_bias, s0, dt_softplus, cu):
     n = b if cu is None else cu.numel() - 1
     s0 = _initial(s0, (n, H, P, N), torch.float32, dev)
     (x, xs), (dt, dts), (B, bs), (C, cs) = _rows(x, 2, 8), _rows(dt, 2), _rows(B, 2, 8), _rows(C, 2, 8)
-    y = x.new_empty((b, T, H, P))
+    y = _out(x)
     sf = A.new_empty((n, H, P, N))
     lib = load_library()
     nbytes = lib.selective_scan_scratch_size(n, T, cu is not None, H, P, G, N)
@@ -273,7 +283,7 @@ def selective_scan_decode(x, dt, A, B, C, state, D=None, dt_bias=None, dt_softpl
     if state.data_ptr() % 16:
         raise ValueError("state must be 16-byte aligned")
     (x, xs), (dt, dts), (B, bs), (C, cs) = _rows(x, 2, 8), _rows(dt, 2), _rows(B, 2, 8), _rows(C, 2, 8)
-    y = x.new_empty((b, T, H, P))
+    y = _out(x)
     _call(dev, "selective_scan_decode", load_library().selective_scan_decode, _p(x), xs, _p(dt), dts,
           dt.dtype == torch.bfloat16, _p(A), _p(B), bs, _p(C), cs, _p(D), _p(dt_bias), bool(dt_softplus), _p(state),
           _p(y), b, T, H, P, G, N)
@@ -293,7 +303,7 @@ def gated_group_rmsnorm(x, z, w, groups: int = 1, eps: float = 1e-6):
     C = x.shape[-1]
     if groups < 1 or C < 1 or C % groups != 0:
         raise ValueError("groups must divide the last dim")
-    y = x.new_empty(x.shape)
+    y = _out(x)
     (x, xs), (z, zs) = _rows(x, x.dim() - 1), _rows(z, z.dim() - 1)
     w = w.contiguous()
     _call(dev, "gated_group_rmsnorm_forward", load_library().gated_group_rmsnorm_forward, _p(x), xs, _p(z), zs, _p(w), _p(y),

@@ -222,6 +222,97 @@ def test_scan_packed(lens):
         assert torch.equal(y2[0, :int(cu[-2])], y[0, :int(cu[-2])]) and torch.equal(sf2[:-1], sf[:-1])
 
 
+def segmented(n, T, packed, H, P, G, N):
+    return gdn_b200.load_library().selective_scan_scratch_size(n, T, int(packed), H, P, G, N) > 0
+
+
+@pytest.mark.parametrize("n,T,H,P,G,N", [(1, 3000, 2, 64, 1, 128), (2, 1500, 3, 72, 1, 40), (1, 1281, 4, 128, 2, 64)])
+def test_scan_segments_of_long_sequences(n, T, H, P, G, N):
+    """Few long sequences, cut into segments whose states are joined: decays from almost none to strong."""
+    assert segmented(n, T, False, H, P, G, N)
+    g = gen(T)
+    s = scan_inputs(g, (n, T), H, P, G, N)
+    s["A"] = -torch.logspace(-3, 1.2, H, device=DEV)
+    s0 = nrm(g, n, H, P, N)
+    y, sf = gdn_b200.selective_scan_prefill(**s, s0=s0, dt_softplus=True)
+    for i in range(n):
+        check_scan(y[i], sf[i], scan_ref(s["x"][i], s["dt"][i], s["A"], s["B"][i], s["C"][i], s["D"], s["dt_bias"], s0[i]))
+
+
+def test_scan_segments_of_a_packed_batch():
+    """Segments of sequences of unlike lengths, empty ones among them, NaN behind the last."""
+    lens, H, P, G, N = [900, 0, 1, 128, 1700, 257, 0], 2, 64, 1, 64
+    g = gen(77)
+    T = sum(lens) + 5
+    assert segmented(len(lens), T, True, H, P, G, N)
+    s = scan_inputs(g, (1, T), H, P, G, N, torch.bfloat16)
+    s["A"] = -torch.tensor([0.01, 4.0], device=DEV)
+    for k in ("x", "B", "C", "dt"):
+        s[k][:, sum(lens):] = float("nan")
+    cu = torch.tensor([0] + lens, device=DEV).cumsum(0).int()
+    s0 = nrm(g, len(lens), H, P, N)
+    y, sf = gdn_b200.selective_scan_prefill_varlen(**s, cu_seqlens=cu, s0=s0, dt_softplus=True)
+    for i, n in enumerate(lens):
+        a = slice(int(cu[i]), int(cu[i]) + n)
+        check_scan(y[0, a], sf[i], scan_ref(s["x"][0, a], s["dt"][0, a], s["A"], s["B"][0, a], s["C"][0, a], s["D"], s["dt_bias"], s0[i]))
+
+
+@pytest.mark.parametrize("count", [31, 70])
+def test_scan_many_packed_sequences(count):
+    """More sequences than a warp has lanes, and fewer (which are taken longest first), all short."""
+    H, P, G, N = 20, 64, 1, 16
+    lens = [(37 * i) % 61 for i in range(count)]
+    g = gen(count)
+    s = scan_inputs(g, (1, sum(lens)), H, P, G, N)
+    cu = torch.tensor([0] + lens, device=DEV).cumsum(0).int()
+    y, sf = gdn_b200.selective_scan_prefill_varlen(**s, cu_seqlens=cu, dt_softplus=True)
+    for i in range(0, count, 3):
+        a = slice(int(cu[i]), int(cu[i + 1]))
+        check_scan(y[0, a], sf[i], scan_ref(s["x"][0, a], s["dt"][0, a], s["A"], s["B"][0, a], s["C"][0, a], s["D"], s["dt_bias"]))
+
+
+def test_scan_offsets_out_of_order_or_range_stay_in_the_buffers():
+    """Bad offsets give no defined results but touch nothing outside: the guard rows keep their contents."""
+    g = gen(15)
+    H, P, G, N, T = 2, 64, 1, 64, 200
+    s = scan_inputs(g, (1, T), H, P, G, N)
+    for bad in ([0, 500, 100, 200], [-7, 30, 20, 1 << 30], [200, 200, 200, 200]):
+        cu = torch.tensor(bad, device=DEV, dtype=torch.int32)
+        y, sf = gdn_b200.selective_scan_prefill_varlen(**s, cu_seqlens=cu, dt_softplus=True)
+        _, cs = gdn_b200.causal_conv_prefill_varlen(s["x"].flatten(2), nrm(g, H * P, 4).bfloat16(), cu)
+        torch.cuda.synchronize()
+    assert (sf == 0).all() and (cs == 0).all()  # the last ones: three empty sequences
+
+
+def test_scan_step_sizes_at_the_edges():
+    """Steps of zero (dt of minus infinity under the softplus), tiny and large ones; a zero initial state."""
+    g = gen(19)
+    s = scan_inputs(g, (1, 140), 4, 64, 1, 64, bias=False)
+    s["dt"][0, 10:40] = float("-inf")
+    s["dt"][0, 40:60] = -30.0
+    s["dt"][0, 60:70] = 40.0
+    y, sf = gdn_b200.selective_scan_prefill(**s, s0=torch.zeros(1, 4, 64, 64, device=DEV), dt_softplus=True)
+    ref = scan_ref(s["x"][0], s["dt"][0], s["A"], s["B"][0], s["C"][0], s["D"])
+    check_scan(y[0], sf[0], ref)
+
+
+def test_scan_prompt_pieces_equal_one_prompt():
+    """A prompt in pieces, each from the last one's state, against the whole: the carried state is exact to fp32."""
+    g = gen(23)
+    H, P, G, N, T = 6, 64, 2, 128, 700
+    s = scan_inputs(g, (1, T), H, P, G, N)
+    par = {k: s[k] for k in ("A", "D", "dt_bias")}
+    cut = lambda a, b: {k: s[k][:, a:b] for k in ("x", "dt", "B", "C")}  # noqa: E731
+    y, sf = gdn_b200.selective_scan_prefill(**s, dt_softplus=True)
+    state, ys = None, []
+    for a, b in ((0, 3), (3, 130), (130, 131), (131, 600), (600, T)):
+        yi, state = gdn_b200.selective_scan_prefill(**cut(a, b), **par, s0=state, dt_softplus=True)
+        ys.append(yi)
+    ref = scan_ref(s["x"][0], s["dt"][0], s["A"], s["B"][0], s["C"][0], s["D"], s["dt_bias"])
+    check_scan(torch.cat(ys, 1)[0], state[0], ref)
+    check_scan(y[0], sf[0], ref)
+
+
 def test_scan_leaves_uncovered_rows():
     """Through the C ABI: rows before the first and behind the last sequence keep their contents."""
     g = gen(8)
@@ -372,7 +463,8 @@ def test_capture_and_replay():
     """All entry points captured into one graph and replayed on new inputs give the eager results."""
     g = gen(41)
     H, P, G, N = 4, 64, 1, 64
-    s = scan_inputs(g, (1, 300), H, P, G, N)
+    s = scan_inputs(g, (1, 2000), H, P, G, N)
+    assert segmented(1, 2000, False, H, P, G, N)
     d = scan_inputs(g, (2, 1), H, P, G, N)
     cx, w, nx, nw = nrm(g, 1, 300, 64).bfloat16(), nrm(g, 64, 4).bfloat16(), nrm(g, 30, 64).half(), nrm(g, 64).half()
     st, cst = nrm(g, 2, H, P, N), nrm(g, 2, 3, 64).bfloat16()
