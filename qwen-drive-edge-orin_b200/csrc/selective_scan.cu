@@ -12,8 +12,10 @@
 namespace gdn {
 namespace ssm {
 
-// Up to this many tokens a prompt runs token by token.
-constexpr int STEP_TOKENS = 6;
+// Up to this many tokens a prompt runs token by token. Measured (64 heads of 64, state 128, 64 sequences):
+// 115 us at 8 tokens and 197 at 16 against 194 for one chunk; one sequence of 24 heads: 6.0 and 10.3
+// against 9.8.
+constexpr int STEP_TOKENS = 15;
 
 static int sm_count() {
     static std::atomic<int> known[64] = {};  // per device; threads that race here store the same value

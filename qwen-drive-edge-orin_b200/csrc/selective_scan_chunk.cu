@@ -1075,21 +1075,23 @@ ChunkPlan plan_scan_chunks(int N, int T, bool packed, int H, int P, int G, int s
     pl.segments = N;
     const int64_t rows = packed ? T : (int64_t)N * T;
     const int64_t chunks = N > 0 ? (rows / N + CH - 1) / CH : 0;  // of the mean sequence
-    // Wave model. Measured on B200: an output pass takes about 4.1 us per chunk and pair and a state pass
-    // 1.1, a CTA's start and end about 4 us and the entry state 0.3 per earlier segment, the second launch 3 us.
-    // Segments pay where the (sequence, pair) units alone leave SMs idle. A packed batch's longest sequence
-    // is taken as twice the mean (the longest ones start first).
+    // Wave model, measured on B200: an output pass takes 4.2 us per chunk and pair and 9.5 for a CTA's start
+    // and end, a state pass 1.8 and 5, the entry states 5. Segments pay where the (sequence, pair) units
+    // alone leave SMs idle (65536 tokens over 8 slots: 2.2 ms in one pass, 103 us in 37 segments). A
+    // packed batch's longest sequence is taken as twice the mean (the longest ones start first).
+    constexpr double OUT = 4.2, OUT_FIXED = 9.5, STATE = 1.8, STATE_FIXED = 5.0, ENTRY = 5.0;
     const int64_t ctas = (int64_t)N * pl.units;
     auto waves = [&](int64_t n) { return (double)((n + sms - 1) / sms); };
-    double best = waves(ctas) * (4.1 * chunks + 4.0);
+    const double one = OUT * chunks + OUT_FIXED;
+    double best = waves(ctas) * one;
     if (packed && N > 1) {
-        const double spread = (double)ctas * (4.1 * chunks + 4.0) / sms + 4.1 * chunks / 2, longest = 2 * 4.1 * chunks + 4.0;
+        const double spread = ctas * one / sms + OUT * chunks / 2, longest = 2 * OUT * chunks + OUT_FIXED;
         best = spread > longest ? spread : longest;
     }
     for (int64_t s = 2; s <= chunks && s <= 64 && ctas * (s - 1) < 4 * sms; ++s) {
         const int64_t per = (chunks + s - 1) / s, cut = (chunks + per - 1) / per;
         if (cut < 2) continue;
-        const double t = waves(ctas * cut) * (4.1 * per + 4.0 + 0.15 * cut) + waves(ctas * (cut - 1)) * (1.1 * per + 4.0) + 3.0;
+        const double t = waves(ctas * cut) * (OUT * per + OUT_FIXED) + waves(ctas * (cut - 1)) * (STATE * per + STATE_FIXED) + ENTRY;
         if (t < best) {
             best = t;
             pl.seg_tokens = (int)(per * CH);
