@@ -19,7 +19,7 @@
 //   warp 17     every TMA load and the TMA stores of the output tiles; warp 18 the gates
 //
 // Precision. G and all sums are fp32. M and the state operand of C S^T are rounded to bf16 once (y is
-// a bf16 output: together 1.0 of its own rounding error). The state itself is an fp32 output and carries
+// a bf16 output, and each of its terms is off by at most one more rounding of that size). The state itself is an fp32 output and carries
 // over thousands of tokens: X' is split exactly into three bf16 terms (8 + 8 + 8 bits of an fp32 value),
 // so its products are those of fp32 operands.
 //
@@ -29,10 +29,19 @@
 // (below: an exponential per element). (A third way was tried and left out: the row factors taken out of
 // M and applied to the finished row where a chunk decays by less than 2^64; no faster.)
 //
-// Bound: shared memory, which feeds the MMAs' operands besides everything else (128 bytes a cycle and SM:
-// an MMA of 128 x 128 x 16 with both operands there takes all of it). So the two operands that the warps
-// form, M and X'^T, are in TMEM: with X' in shared memory (8 instead of 4 KB per MMA, and written there)
-// the same chunk took 5.9 K cycles of its bandwidth instead of 4.6 K.
+// Measured on B200: 7.2 K cycles (4.2 us) per chunk and slot pair with one CTA on every SM, against 1.5 us for
+// the pair's 64 KB of x and y at the copy bandwidth; 8 x 4096 tokens of 64 heads of 64 in 264 us (256 CTAs in
+// two waves), token by token 6.3 ms. No unit is full (tensor pipe 50%, shared memory 49%, issue slots 66% on the
+// fullest SM): two loops of dependent steps take the same time, G - M - scaling of y - M X - next G, and state
+// operand - output tile - X'^T - state product. What led here:
+//   - shared memory feeds the MMAs' operands besides everything else (an MMA of 128 x 128 x 16 with both
+//     operands there takes all of its 128 bytes a cycle), so the two operands that the warps form, M and X'^T,
+//     are in TMEM;
+//   - the kernel is sensitive to instruction fetch: with 90 instead of 63 KB of code the same steps took 315
+//     instead of 262 us. So there is one copy of each step and loops stay rolled;
+//   - plain pointers into shared memory load through the generic path (304 against 269 us).
+// No faster, and left out: twenty-four working warps, M shared by all sixteen, all of X'^T in warps 0-7, three
+// x buffers with one B buffer.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -109,7 +118,7 @@ enum {
     B_PF = 22, B_PE = 24,  // gates
     B_YS = 26,             // output tile written, per slot and buffer
     B_DR = 30,             // every MMA of an issuing thread done (exit)
-    B_BE = 32,
+    B_BE = 32,             // B buffers read
     NBARS = 34
 };
 static_assert(MISC_BAR + 8 * NBARS <= MISC_TMEM, "barriers overlap the TMEM address word");
@@ -490,7 +499,10 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
 #pragma unroll 1
             for (int hf = 0; hf < 2; ++hf) {
                 float v[32];
+                uint32_t x[16];
                 ptx::tmem_ld32(tm_y + 32 * hf, v);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) ld_shared_v4(xt ^ ((4 * hf + c) << 4), x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
                 ptx::tmem_wait_ld();
                 if (hf == 1) {
                     ptx::tc_fence_before();
@@ -500,11 +512,10 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 for (int c = 0; c < 4; ++c) {
                     const uint32_t at = xt ^ ((4 * hf + c) << 4);
                     uint32_t u[4];
-                    ld_shared_v4(at, u[0], u[1], u[2], u[3]);
 #pragma unroll
                     for (int t = 0; t < 4; ++t) {
                         float x0, x1;
-                        f2_unpack(f2_fma(f2_pack(__uint_as_float(u[t] << 16), __uint_as_float(u[t] & 0xFFFF0000u)), dd,
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(x[4 * c + t] << 16), __uint_as_float(x[4 * c + t] & 0xFFFF0000u)), dd,
                                          f2_pack(v[8 * c + 2 * t], v[8 * c + 2 * t + 1])),
                                   x0, x1);
                         u[t] = pack_bf16(x0, x1);
