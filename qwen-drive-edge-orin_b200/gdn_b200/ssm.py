@@ -18,6 +18,7 @@ __all__ = ["causal_conv_prefill", "causal_conv_prefill_varlen", "causal_conv_dec
            "selective_scan_prefill_varlen", "selective_scan_decode", "gated_group_rmsnorm"]
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_MAX_GRID = 65535  # sequences and heads of a scan are grid dimensions
 # the current stream's handle without a Stream object: a single-token call is bound by its host time
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
@@ -229,6 +230,8 @@ def _check_scan(x, dt, A, B, C, D, dt_bias, packed=False):
         raise ValueError("P and N must be multiples of 8 up to 128")
     if packed and b != 1:
         raise ValueError("varlen inputs are packed: B must be 1")
+    if b > _MAX_GRID or H > _MAX_GRID:
+        raise ValueError(f"at most {_MAX_GRID} sequences and heads are supported")
     A = _vector(A, H, torch.float32, "A", dev)
     D = _vector(D, H, torch.float32, "D", dev)
     dt_bias = _vector(dt_bias, H, torch.float32, "dt_bias", dev)
@@ -240,6 +243,8 @@ def _scan_prefill(x, dt, A, B, C, D, dt_bias, s0, dt_softplus, cu):
     if cu is not None:
         cu = _offsets(cu, dev)
     n = b if cu is None else cu.numel() - 1
+    if n > _MAX_GRID:
+        raise ValueError(f"at most {_MAX_GRID} sequences and heads are supported")
     s0 = _initial(s0, (n, H, P, N), torch.float32, dev)
     (x, xs), (dt, dts), (B, bs), (C, cs) = _rows(x, 2, 8), _rows(dt, 2), _rows(B, 2, 8), _rows(C, 2, 8)
     y = _out(x)
@@ -259,7 +264,10 @@ def selective_scan_prefill(x, dt, A, B, C, D=None, dt_bias=None, s0=None, dt_sof
     Per head h of group g = h // (H // G), with d = dt + dt_bias (softplus'ed if ``dt_softplus``):
         S <- exp(d A) S + d x B^T;   y = S C + D x.
     x bf16 [B,T,H,P], dt fp32 or bf16 [B,T,H], B/C bf16 [B,T,G,N], A, D, dt_bias fp32 [H], initial
-    state s0 fp32 [B,H,P,N] or zeros. P and N are multiples of 8 up to 128; d A <= 0 is expected.
+    state s0 fp32 [B,H,P,N] or zeros. P and N are multiples of 8 up to 128, B and H at most 65535, and
+    d A <= 0. A token with d = 0 (dt of minus infinity under the softplus) leaves the state as it is, so
+    padding in front of or between tokens is possible. An x that is not finite
+    makes its channel's outputs NaN from the start of its 128 tokens (of its sequence) on.
     """
     return _scan_prefill(x, dt, A, B, C, D, dt_bias, s0, dt_softplus, None)
 

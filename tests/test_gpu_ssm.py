@@ -296,6 +296,60 @@ def test_scan_step_sizes_at_the_edges():
     check_scan(y[0], sf[0], ref)
 
 
+@pytest.mark.parametrize("size", [300.0, 1e4, 3e6, 1e20])
+@pytest.mark.parametrize("kept", [False, True])
+def test_scan_after_tokens_that_end_the_past(size, kept):
+    """A step so large that nothing before it is left, once with its own input and once with none: the
+    tokens behind it in its block see the small steps between them."""
+    g = gen(23)
+    s = scan_inputs(g, (1, 300), 4, 64, 1, 64, bias=False)
+    s["dt"] = 0.02 + 0.1 * s["dt"].abs()
+    s["A"] = torch.tensor([-1.0, -0.2, -3.0, -0.01], device=DEV)
+    for t in (37, 100, 101, 128, 255):
+        s["dt"][0, t] = size / s["A"].abs()
+        if not kept:
+            s["x"][0, t] = 0
+    y, sf = gdn_b200.selective_scan_prefill(**s)
+    check_scan(y[0], sf[0], scan_ref(s["x"][0], s["dt"][0], s["A"], s["B"][0], s["C"][0], s["D"], dt_softplus=False))
+
+
+@pytest.mark.parametrize("name,value,first", [("x", math.nan, 128), ("x", math.inf, 128), ("B", math.nan, 200), ("B", -math.inf, 200),
+                                              ("C", math.nan, 200), ("dt", math.nan, 200), ("dt", math.inf, 200)])
+def test_scan_values_that_are_not_finite_leave_earlier_tokens(name, value, first):
+    g = gen(29)
+    s = scan_inputs(g, (1, 300), 2, 64, 1, 64)
+    ref = scan_ref(s["x"][0, :first], s["dt"][0, :first], s["A"], s["B"][0, :first], s["C"][0, :first], s["D"], s["dt_bias"])
+    _, clean = gdn_b200.selective_scan_prefill(**{k: v[:, :first] if v.dim() > 1 else v for k, v in s.items()}, dt_softplus=True)
+    s[name][0, 200] = value
+    y, _ = gdn_b200.selective_scan_prefill(**s, dt_softplus=True)
+    check_scan(y[0, :first], clean[0], ref)
+    assert not torch.isfinite(y[0, 200]).any()
+
+
+@pytest.mark.parametrize("T", [14, 15, 16, 17])
+def test_scan_short_prompts(T):
+    g = gen(T)
+    s = scan_inputs(g, (3, T), 4, 64, 2, 128)
+    s0 = nrm(g, 3, 4, 64, 128)
+    y, sf = gdn_b200.selective_scan_prefill(**s, s0=s0, dt_softplus=True)
+    for i in range(3):
+        check_scan(y[i], sf[i], scan_ref(s["x"][i], s["dt"][i], s["A"], s["B"][i], s["C"][i], s["D"], s["dt_bias"], s0[i]))
+
+
+def test_scan_refuses_more_sequences_or_heads_than_a_grid_holds():
+    e = lambda *shape: torch.empty(*shape, device=DEV, dtype=torch.bfloat16)
+    f = lambda *shape: torch.empty(*shape, device=DEV)
+    for b, H in ((65536, 1), (1, 65536)):
+        args = (e(b, 1, H, 8), f(b, 1, H), f(H), e(b, 1, 1, 8), e(b, 1, 1, 8))
+        with pytest.raises(ValueError):
+            gdn_b200.selective_scan_prefill(*args)
+        with pytest.raises(ValueError):
+            gdn_b200.selective_scan_decode(*args, f(b, H, 8, 8))
+    with pytest.raises(ValueError):
+        gdn_b200.selective_scan_prefill_varlen(e(1, 1, 1, 8), f(1, 1, 1), f(1), e(1, 1, 1, 8), e(1, 1, 1, 8),
+                                               torch.zeros(65537, dtype=torch.int32, device=DEV))
+
+
 def test_scan_prompt_pieces_equal_one_prompt():
     """A prompt in pieces, each from the last one's state, against the whole: the carried state is exact to fp32."""
     g = gen(23)
