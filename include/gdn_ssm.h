@@ -55,7 +55,7 @@ cudaError_t causal_conv_decode(const void* x, int64_t x_stride, const void* w, c
  * channel's outputs NaN from the start of its 128 tokens (counted from the sequence's start) on, not
  * from its own token on; no value of any input reaches another sequence.
  * workspace: at least 256 bytes, zero before its first use, whose first word is the status word
- * (deltanet_read_status); calls may share it. scratch: selective_scan_scratch_size(...) bytes for the
+ * (deltanet_read_status: 0, or bits 0 and 16 where a bounded wait of the scan ran out); calls may share it. scratch: selective_scan_scratch_size(...) bytes for the
  * same sizes on the same device, 256-byte aligned (NULL where that is 0); calls that may overlap in
  * time need scratch of their own. */
 size_t selective_scan_scratch_size(int N, int T, int packed, int H, int P, int G, int n_state);
