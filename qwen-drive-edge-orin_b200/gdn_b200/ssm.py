@@ -99,6 +99,13 @@ def _rows(t, lead, align=1):
     return t, stride
 
 
+def _wide_rows(t, lead, width, align=1):
+    """``_rows`` of a t whose rows are known to be ``width`` wide: a contiguous one takes no walk over its dims."""
+    if t.is_contiguous() and (align == 1 or (width % align == 0 and t.data_ptr() % (align * t.element_size()) == 0)):
+        return t, width
+    return _rows(t, lead, align)
+
+
 def _packed_rows(t, width, align):
     t = t.contiguous()
     if t.data_ptr() % (align * t.element_size()):
@@ -165,7 +172,7 @@ def _conv_prefill(x, w, bias, s0, silu, cu):
         cu = _offsets(cu, dev)
     n = B if cu is None else cu.numel() - 1
     s0 = _initial(s0, (n, W - 1, C), x.dtype, dev)
-    x, stride = _rows(x, 2)
+    x, stride = _wide_rows(x, 2, C)
     w = w.contiguous()
     y = _out(x)
     sf = x.new_empty((n, W - 1, C))
@@ -200,10 +207,10 @@ def causal_conv_decode(x, w, state, bias=None, silu: bool = True):
     dev, bias = _check_conv(x, w, bias)
     B, T, C = x.shape
     W = w.shape[1]
-    if state.dtype != x.dtype or not state.is_contiguous() or tuple(state.shape) != (B, W - 1, C):
+    if state.dtype != x.dtype or not state.is_contiguous() or state.shape != (B, W - 1, C):
         raise ValueError(f"state must be a contiguous tensor of x's dtype and shape {(B, W - 1, C)}")
     _on_one_device(x, state)
-    x, stride = _rows(x, 2)
+    x, stride = _wide_rows(x, 2, C)
     w = w.contiguous()
     y = _out(x)
     _call(dev, "causal_conv_decode", load_library().causal_conv_decode, _p(x), stride, _p(w), _p(bias), _p(state), _p(y),
@@ -221,8 +228,9 @@ def _check_scan(x, dt, A, B, C, D, dt_bias, packed=False):
     if x.dim() != 4 or B.dim() != 4 or C.dim() != 4 or dt.dim() != 3:
         raise ValueError("bad ranks: x must be 4-D [B,T,H,P], B/C 4-D [B,T,G,N], dt 3-D [B,T,H]")
     b, T, H, P = x.shape
-    G, N = B.shape[2], B.shape[3]
-    if B.shape[:2] != (b, T) or C.shape != B.shape or dt.shape != (b, T, H):
+    bshape = B.shape
+    bb, bt, G, N = bshape
+    if bb != b or bt != T or C.shape != bshape or dt.shape != (b, T, H):
         raise ValueError("shape mismatch between x/dt/B/C")
     if G < 1 or H < 1 or H % G != 0:
         raise ValueError("H must be a multiple of G")
@@ -246,7 +254,8 @@ def _scan_prefill(x, dt, A, B, C, D, dt_bias, s0, dt_softplus, cu):
     if n > _MAX_GRID:
         raise ValueError(f"at most {_MAX_GRID} sequences and heads are supported")
     s0 = _initial(s0, (n, H, P, N), torch.float32, dev)
-    (x, xs), (dt, dts), (B, bs), (C, cs) = _rows(x, 2, 8), _rows(dt, 2), _rows(B, 2, 8), _rows(C, 2, 8)
+    (x, xs), (dt, dts) = _wide_rows(x, 2, H * P, 8), _wide_rows(dt, 2, H)
+    (B, bs), (C, cs) = _wide_rows(B, 2, G * N, 8), _wide_rows(C, 2, G * N, 8)
     y = _out(x)
     sf = A.new_empty((n, H, P, N))
     lib = load_library()
@@ -285,12 +294,13 @@ def selective_scan_decode(x, dt, A, B, C, state, D=None, dt_bias=None, dt_softpl
     """The scan of the next token(s) x [B,T,H,P] (T usually 1), shapes as in ``selective_scan_prefill``:
     returns y; the fp32 ``state`` [B,H,P,N] (e.g. a prefill's final state) is updated in place."""
     dev, (b, T, H, P, G, N), A, D, dt_bias = _check_scan(x, dt, A, B, C, D, dt_bias)
-    if state.dtype != torch.float32 or not state.is_contiguous() or tuple(state.shape) != (b, H, P, N):
+    if state.dtype != torch.float32 or not state.is_contiguous() or state.shape != (b, H, P, N):
         raise ValueError("state must be a contiguous fp32 [B, H, P, N] tensor")
     _on_one_device(x, state)
     if state.data_ptr() % 16:
         raise ValueError("state must be 16-byte aligned")
-    (x, xs), (dt, dts), (B, bs), (C, cs) = _rows(x, 2, 8), _rows(dt, 2), _rows(B, 2, 8), _rows(C, 2, 8)
+    (x, xs), (dt, dts) = _wide_rows(x, 2, H * P, 8), _wide_rows(dt, 2, H)
+    (B, bs), (C, cs) = _wide_rows(B, 2, G * N, 8), _wide_rows(C, 2, G * N, 8)
     y = _out(x)
     _call(dev, "selective_scan_decode", load_library().selective_scan_decode, _p(x), xs, _p(dt), dts,
           dt.dtype == torch.bfloat16, _p(A), _p(B), bs, _p(C), cs, _p(D), _p(dt_bias), bool(dt_softplus), _p(state),
@@ -312,7 +322,8 @@ def gated_group_rmsnorm(x, z, w, groups: int = 1, eps: float = 1e-6):
     if groups < 1 or C < 1 or C % groups != 0:
         raise ValueError("groups must divide the last dim")
     y = _out(x)
-    (x, xs), (z, zs) = _rows(x, x.dim() - 1), _rows(z, z.dim() - 1)
+    lead = x.dim() - 1
+    (x, xs), (z, zs) = _wide_rows(x, lead, C), _wide_rows(z, lead, C)
     w = w.contiguous()
     _call(dev, "gated_group_rmsnorm_forward", load_library().gated_group_rmsnorm_forward, _p(x), xs, _p(z), zs, _p(w), _p(y),
           x.numel() // C, C, int(groups), float(eps), _DTYPES[x.dtype])
