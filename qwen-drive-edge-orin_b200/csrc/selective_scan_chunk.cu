@@ -31,8 +31,8 @@
 //
 // Measured on B200: 7.2 K cycles (4.2 us) per chunk and slot pair with one CTA on every SM, against 1.5 us for
 // the pair's 64 KB of x and y at the copy bandwidth; 8 x 4096 tokens of 64 heads of 64 in 264 us (256 CTAs in
-// two waves), token by token 6.3 ms. No unit is full (tensor pipe 50%, shared memory 49%, issue slots 66% on the
-// fullest SM): two loops of dependent steps take the same time, G - M - scaling of y - M X - next G, and state
+// two waves), token by token 6.3 ms. No unit is full (on the fullest SM: tensor pipe 50%, shared memory 48%;
+// issue slots 66% on its fullest quarter): two loops of dependent steps take the same time, G - M - scaling of y - M X - next G, and state
 // operand - output tile - X'^T - state product. What led here:
 //   - shared memory feeds the MMAs' operands besides everything else (an MMA of 128 x 128 x 16 with both
 //     operands there takes all of its 128 bytes a cycle), so the two operands that the warps form, M and X'^T,
