@@ -133,6 +133,7 @@ struct ChunkParams {
     int pairs;         // slot pairs per group
     int units;         // G * pairs
     int seg_tokens;    // tokens per segment (a multiple of 128), 0: one segment per sequence
+    int segments;      // segments that part and part_log have room for
 };
 
 // The rest of a wait whose first test failed, out of line (the kernel has some thirty waits and is
@@ -997,7 +998,10 @@ __global__ void __launch_bounds__(256) scan_entry_kernel(const __grid_constant__
         if (lane == 0) found[0] = first, found[1] = count;
     }
     __syncthreads();
-    const int first = found[0], count = found[1];
+    // The scratch holds the segments of sequences that do not overlap. Offsets that are out of order can make
+    // overlapping ones of the clamped ranges: what lies behind the scratch is no segment of this call. (No
+    // overflow: a call is cut only with fewer than 4 x 148 sequences and at most 64 segments of a mean one.)
+    const int first = found[0], count = min(found[1], p.segments - first);
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();  // the state pass's results
     if (count < 2) return;
@@ -1134,6 +1138,7 @@ cudaError_t launch_scan_chunks(const ScanArgs& a, const ChunkPlan& pl, int64_t r
     p.pairs = pl.pairs;
     p.units = pl.units;
     p.seg_tokens = pl.seg_tokens;
+    p.segments = (int)pl.segments;
     const int64_t ctas = pl.segments * pl.units;
     if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
     if (pl.seg_tokens == 0) {

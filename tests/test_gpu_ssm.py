@@ -284,6 +284,41 @@ def test_scan_offsets_out_of_order_or_range_stay_in_the_buffers():
     assert (sf == 0).all() and (cs == 0).all()  # the last ones: three empty sequences
 
 
+@pytest.mark.parametrize("bad", [[0, 3000, 0, 3000], [0, 3000, 500, 3000], [0, 3000, -5, 1 << 30, 0, 3000], [3000, 0, 3000, 0, 3000],
+                                 [0, 1000, 2000, 3000]])
+def test_scan_segments_of_offsets_out_of_order_stay_in_the_scratch(bad):
+    """Offsets out of order make overlapping sequences: more segments than the scratch has room for. Through the
+    C ABI, with guard words around the scratch, the outputs and the final states."""
+    g = gen(16)
+    H, P, G, N, T, n, pad = 2, 64, 1, 128, 3000, len(bad) - 1, 1 << 16
+    lib = gdn_b200.load_library()
+    nbytes = lib.selective_scan_scratch_size(n, T, 1, H, P, G, N)
+    assert nbytes > 0
+    s = scan_inputs(g, (1, T), H, P, G, N)
+    cu = torch.tensor(bad, device=DEV, dtype=torch.int32)
+    # enough behind the scratch for every sequence to have T tokens in segments of one chunk
+    behind = n * (T // 128 + 1) * H * 64 * 128 * 4
+    scratch = torch.full((nbytes + 256 + behind,), 0x5A, device=DEV, dtype=torch.uint8)
+    y = torch.full((pad + T * H * P + pad,), 7.0, device=DEV, dtype=torch.bfloat16)
+    sf = torch.full((pad + n * H * P * N + pad,), 7.0, device=DEV)
+    ws = torch.zeros(256, dtype=torch.uint8, device=DEV)
+    rc = lib.selective_scan_prefill(s["x"].data_ptr(), H * P, s["dt"].data_ptr(), H, 0, s["A"].data_ptr(), s["B"].data_ptr(), G * N,
+                                    s["C"].data_ptr(), G * N, s["D"].data_ptr(), s["dt_bias"].data_ptr(), 1, None, y[pad:].data_ptr(),
+                                    sf[pad:].data_ptr(), cu.data_ptr(), n, T, H, P, G, N, ws.data_ptr(), 256,
+                                    scratch[256:].data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    torch.cuda.synchronize()
+    assert (scratch[:256] == 0x5A).all() and (scratch[256 + nbytes:] == 0x5A).all()
+    for t, size in ((y, T * H * P), (sf, n * H * P * N)):
+        assert (t[:pad] == 7).all() and (t[pad + size:] == 7).all()
+    assert not ws.any()
+    if bad == sorted(bad):  # in order: the room is enough, and the results are right
+        for i in range(n):
+            a = slice(bad[i], bad[i + 1])
+            check_scan(y[pad:pad + T * H * P].view(T, H, P)[a], sf[pad:pad + n * H * P * N].view(n, H, P, N)[i],
+                       scan_ref(s["x"][0, a], s["dt"][0, a], s["A"], s["B"][0, a], s["C"][0, a], s["D"], s["dt_bias"]))
+
+
 def test_scan_step_sizes_at_the_edges():
     """Steps of zero (dt of minus infinity under the softplus), tiny and large ones; a zero initial state."""
     g = gen(19)
