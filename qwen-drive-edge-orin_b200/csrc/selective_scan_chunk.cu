@@ -25,8 +25,9 @@
 //
 // Decays are kept as base-2 logarithms, relative to 32-token blocks: e^{c_i - c_j} is a row factor times
 // a column factor, one exponential per row and block. Across blocks both are at most 1; inside a block
-// the row factor undoes the column factor beyond the row, which fp32 holds for decays down to 2^-100
-// (below: an exponential per element). (A third way was tried and left out: the row factors taken out of
+// the row factor undoes the column factor beyond the row. fp32 holds both where the block decays by less than
+// 2^100 and no column factor times its step size is below the normal range; the gate warp marks the other
+// blocks, which take an exponential per element. (A third way was tried and left out: the row factors taken out of
 // M and applied to the finished row where a chunk decays by less than 2^64; no faster.)
 //
 // Measured on B200: 7.2 K cycles (4.2 us) per chunk and slot pair with one CTA on every SM, against 1.5 us for
@@ -82,8 +83,9 @@ constexpr uint32_t MISC_TMEM = 344;
 constexpr uint32_t MISC_SEG = 348;                   // the CTA's segment and slots:
 enum { SEG_SEQ, SEG_J, SEG_COUNT, SEG_ROW, SEG_LEN, SEG_HEAD, SEG_TILE = SEG_HEAD + 2, SEG_SECOND = SEG_TILE + 2,
        SEG_GROUP, SEG_WORDS };
+constexpr uint32_t MISC_EXP = 400;                   // [2 buffers][2 slots]: bit b, block b needs an exponential per element
 constexpr uint32_t MISC_BYTES = 448;
-static_assert(MISC_SEG + 4 * SEG_WORDS <= MISC_BYTES, "segment words overflow");
+static_assert(MISC_SEG + 4 * SEG_WORDS <= MISC_EXP && MISC_EXP + 16 <= MISC_BYTES, "segment words overflow");
 constexpr uint32_t CHUNK_SMEM = OFF_MISC + MISC_BYTES + 1024;
 static_assert(CHUNK_SMEM <= 232448, "exceeds the 227 KB per-block shared memory limit");
 
@@ -209,6 +211,7 @@ __device__ __forceinline__ float4 lds4(uint32_t addr) {
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
     return v;
 }
+__device__ __forceinline__ void sts1(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 __device__ __forceinline__ void sts4(uint32_t addr, float4 v) {
     asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
@@ -398,6 +401,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
     // gates and block sums as shared-memory addresses (plain pointers would load through the generic path)
     auto gates = [&](int buf, int s) { return sb + OFF_GATE + (uint32_t)(2 * buf + s) * GATE_BYTES; };
     auto sums = [&](int buf, int s) { return sb + OFF_MISC + MISC_SUMS + (uint32_t)(2 * buf + s) * 16; };
+    auto exps = [&](int buf, int s) { return sb + OFF_MISC + MISC_EXP + (uint32_t)(2 * buf + s) * 4; };
     const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16);  // this warp's TMEM lane quarter
 
     // ---- X'^T (warps 0-15): warpgroup i forms piece i of a chunk, 32 tokens; a thread one slot channel
@@ -631,16 +635,16 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
 #pragma unroll 1
                         for (int s = 0; s < (twin ? 1 : 2); ++s) {
                             const uint32_t gt = gates(buf, s), R = sums(buf, s);
-                            const float ci = lds1(gt + 4 * (GT_C + row)), Rq = lds1(R + 4 * q);
+                            const float ci = lds1(gt + 4 * (GT_C + row));
                             uint32_t o[16];
                             if (b < q) {
                                 float e = ci;
 #pragma unroll 1
                                 for (int m = b + 1; m < q; ++m) e += lds1(R + 4 * m);
                                 form_m<false>(v, o, gt + 4 * (GT_H + 32 * b), ex2f(e), 0);
-                            } else if (Rq > -100.f) {  // the row factor undoes h_j's 2^{R - c_j} beyond i
-                                form_m<true>(v, o, gt + 4 * (GT_H + 32 * b), ex2f(ci - Rq), (2u << lane) - 1u);
-                            } else {  // decays beyond fp32's range inside the block: an exponential per element
+                            } else if (!(__float_as_uint(lds1(exps(buf, s))) >> q & 1)) {  // the row factor undoes h_j's 2^{R - c_j} beyond i
+                                form_m<true>(v, o, gt + 4 * (GT_H + 32 * b), ex2f(ci - lds1(R + 4 * q)), (2u << lane) - 1u);
+                            } else {  // factors beyond fp32's range inside the block: an exponential per element
 #pragma unroll
                                 for (int j = 0; j < 32; j += 4) {
                                     const float4 c4 = lds4(gt + 4 * (GT_C + 32 * q + j)), d4 = lds4(gt + 4 * (GT_D + 32 * q + j));
@@ -950,7 +954,18 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
             sts4(gt + 4 * GT_C, make_float4(left + pre[0], left + pre[1], left + pre[2], left + pre[3]));
             sts4(gt + 4 * GT_W, make_float4(hv[0] * f, hv[1] * f, hv[2] * f, hv[3] * f));
             sts4(gt + 4 * GT_H, make_float4(hv[0], hv[1], hv[2], hv[3]));
-            if (lane == 0) sts4(sums(buf, s), make_float4(R[0], R[1], R[2], R[3]));
+            // (NaN steps and decays count as out of range: the element form keeps them to the tokens behind)
+            bool out = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out |= d[i] != 0.f && !(fabsf(hv[i]) >= 1.17549435e-38f);
+            const unsigned outs = __ballot_sync(0xffffffffu, out);
+            if (lane == 0) {
+                uint32_t e = 0;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) e |= ((outs >> (8 * b) & 0xffu) != 0 || !(R[b] > -100.f)) ? 1u << b : 0u;
+                sts4(sums(buf, s), make_float4(R[0], R[1], R[2], R[3]));
+                sts1(exps(buf, s), __uint_as_float(e));
+            }
             }
             if (k >= 0) warp_arrive(B_PF + buf);
 #pragma unroll

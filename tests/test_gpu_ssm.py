@@ -331,6 +331,24 @@ def test_scan_step_sizes_at_the_edges():
     check_scan(y[0], sf[0], ref)
 
 
+@pytest.mark.parametrize("step", [1e-10, 1e-13, 1e-25, 1e-30])
+@pytest.mark.parametrize("log2", [-60.0, -95.0, -99.5])
+def test_scan_tiny_steps_before_a_strong_decay(step, log2):
+    """Rows between steps so small and, in the same 32 tokens, a decay just within fp32's range: their outputs
+    are small and normal numbers, compared relative to the terms' own size (no D, no initial state)."""
+    g = gen(24)
+    s = scan_inputs(g, (1, 150), 2, 64, 1, 64, bias=False, D=False)
+    s["A"] = torch.tensor([-1.0, -0.5], device=DEV)
+    s["dt"] = step * (1 + torch.rand(1, 150, 2, generator=g, device=DEV))
+    for t in (20, 60, 149):
+        s["dt"][0, t] = log2 * math.log(2.0) / s["A"]
+    y, sf = gdn_b200.selective_scan_prefill(**s)
+    ry, my, S, M = scan_ref(s["x"][0], s["dt"][0], s["A"], s["B"][0], s["C"][0], dt_softplus=False)
+    # the scan's bounds; terms below 2^-126 (the decay's remains) may be lost
+    close(sf[0], S, 2.0 ** -16 * M + 1e-36)
+    close(y[0], ry, 2.0 ** -8 * (ry.abs() + my) * 1.01 + 1e-36 * 64 * 8)
+
+
 @pytest.mark.parametrize("size", [300.0, 1e4, 3e6, 1e20])
 @pytest.mark.parametrize("kept", [False, True])
 def test_scan_after_tokens_that_end_the_past(size, kept):
