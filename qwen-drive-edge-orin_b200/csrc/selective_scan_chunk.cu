@@ -916,10 +916,14 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
             const float A2s = s ? A2[1] : A2[0];
             // log2 decays, clamped: 2^-256 is zero like any smaller factor, and the distances of the tokens
             // behind such a step are differences of sums that hold it (one step of 256 leaves them 2^-16,
-            // a block of 32 of them 2^-11)
+            // a block of 32 of them 2^-11). NaN stays; rows behind the sequence count nothing, whatever A is.
             float t[4], pre[4], suf[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) t[i] = fmaxf(d[i] * A2s, -256.f);
+            for (int i = 0; i < 4; ++i) {
+                t[i] = d[i] * A2s;
+                t[i] = t[i] < -256.f ? -256.f : t[i];
+                t[i] = 4 * lane + i < valid ? t[i] : 0.f;
+            }
             pre[0] = t[0], pre[1] = t[0] + t[1], pre[2] = pre[1] + t[2], pre[3] = pre[2] + t[3];
             suf[3] = 0.f, suf[2] = t[3], suf[1] = t[3] + t[2], suf[0] = suf[1] + t[1];
             // sums over the 8 lanes of a 32-token block, from the left and, for the accuracy of the

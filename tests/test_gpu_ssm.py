@@ -379,6 +379,22 @@ def test_scan_values_that_are_not_finite_leave_earlier_tokens(name, value, first
     assert not torch.isfinite(y[0, 200]).any()
 
 
+@pytest.mark.parametrize("T", [7, 20, 150, 256, 3000])
+def test_scan_decay_rates_of_minus_infinity_and_nan(T):
+    """A rate of minus infinity leaves each token its own input, in a partial chunk too; a NaN makes its head NaN
+    (outputs and state) and no other's."""
+    g = gen(T)
+    s = scan_inputs(g, (1, T), 4, 64, 1, 64)
+    s["A"] = torch.tensor([-math.inf, -1.0, math.nan, -2.0], device=DEV)
+    s0 = nrm(g, 1, 4, 64, 64)
+    y, sf = gdn_b200.selective_scan_prefill(**s, s0=s0, dt_softplus=True)
+    ry, my, S, M = scan_ref(s["x"][0], s["dt"][0], s["A"], s["B"][0], s["C"][0], s["D"], s["dt_bias"], s0[0])
+    for h in (0, 1, 3):
+        check_scan(y[0, :, h], sf[0, h], (ry[:, h], my[:, h], S[h], M[h]))
+    assert torch.isnan(ry[:, 2]).all() and torch.isnan(S[2]).all()
+    assert torch.isnan(y[0, :, 2]).all() and torch.isnan(sf[0, 2]).all()
+
+
 @pytest.mark.parametrize("T", [14, 15, 16, 17])
 def test_scan_short_prompts(T):
     g = gen(T)
