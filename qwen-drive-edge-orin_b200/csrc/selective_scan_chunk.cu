@@ -258,7 +258,7 @@ __device__ __forceinline__ float head(float a) { return __uint_as_float(__float_
 __device__ __forceinline__ void find_segment(const ScanArgs& a, int seg_tokens, int sid, int lane, int& seq, int& j, int& count) {
     seq = sid, j = 0, count = 1;
     if (seg_tokens > 0 && a.cu == nullptr) {
-        count = max(1, (a.T + seg_tokens - 1) / seg_tokens);
+        count = (a.T - 1) / seg_tokens + 1;  // (no sum: T may be near 2^31; a call that is cut has tokens)
         seq = sid / count;
         j = sid - seq * count;
     } else if (seg_tokens == 0 && a.cu != nullptr && a.N <= 32) {  // packed: the longest sequences first
@@ -996,7 +996,7 @@ __global__ void __launch_bounds__(256) scan_entry_kernel(const __grid_constant__
     if (threadIdx.x < 32) {
         int first = 0, count = 1;
         if (a.cu == nullptr) {
-            count = max(1, (a.T + p.seg_tokens - 1) / p.seg_tokens);
+            count = (a.T - 1) / p.seg_tokens + 1;
             first = seq * count;
         } else {
             for (int s0 = 0; s0 <= seq; s0 += 32) {  // segments of the sequences before
@@ -1131,7 +1131,7 @@ ChunkPlan plan_scan_chunks(int N, int T, bool packed, int H, int P, int G, int s
         if (t < best) {
             best = t;
             pl.seg_tokens = (int)(per * CH);
-            pl.segments = packed ? (int64_t)T / pl.seg_tokens + N : (int64_t)N * ((T + pl.seg_tokens - 1) / pl.seg_tokens);
+            pl.segments = packed ? (int64_t)T / pl.seg_tokens + N : (int64_t)N * ((T - 1) / pl.seg_tokens + 1);
         }
     }
     const int64_t parts = pl.seg_tokens > 0 ? pl.segments * pl.units * 2 : 0;

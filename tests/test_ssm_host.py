@@ -54,6 +54,18 @@ def _scan(**kw):
     return gdn_b200.load_library().selective_scan_prefill(*a.values(), None)
 
 
+@pytest.mark.parametrize("T", [(1 << 31) - 129, 2_120_000_000, 1 << 24])
+@pytest.mark.parametrize("n", [1, 2])
+def test_scan_scratch_of_the_longest_sequences(T, n):
+    """Segments of sequences up to the 2^31 - 129 token rows that a call may have: 64 KB of states (128 rows of 128
+    fp32) and two log decays each, at most 64 segments a sequence."""
+    T //= n
+    size = gdn_b200.load_library().selective_scan_scratch_size(n, T, 0, 1, 8, 1, 8)
+    segments = size // 65536
+    assert n < segments <= 64 * n and segments % n == 0
+    assert size == segments * 65536 + -(-segments * 8 // 256) * 256
+
+
 def _scan_decode(**kw):
     a = dict(x=P, xs=128, dt=P, dts=2, dtb=0, A=P, B=P, bs=128, C=P, cs=128, D=None, bias=None, sp=1, state=P, y=P,
              N=1, T=4, H=2, P=64, G=1, NS=128)
