@@ -23,13 +23,17 @@ _MAX_GRID = 65535  # sequences and heads of a scan are grid dimensions
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
+def _on(dev, fn, *args):
+    """fn(*args) with device index ``dev`` current."""
+    if dev == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)
+
+
 def _call(dev, what, fn, *args):
     """fn(*args, stream) on torch's current stream of device index ``dev``."""
-    if dev == torch.cuda.current_device():
-        code = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            code = fn(*args, _raw_stream(dev))
+    code = _on(dev, fn, *args, _raw_stream(dev))
     if code:
         _check(code, what)
 
@@ -259,7 +263,7 @@ def _scan_prefill(x, dt, A, B, C, D, dt_bias, s0, dt_softplus, cu):
     y = _out(x)
     sf = A.new_empty((n, H, P, N))
     lib = load_library()
-    nbytes = lib.selective_scan_scratch_size(n, T, cu is not None, H, P, G, N)
+    nbytes = _on(dev, lib.selective_scan_scratch_size, n, T, cu is not None, H, P, G, N)  # (plans for the current device)
     scratch = A.new_empty(nbytes // 4) if nbytes else None
     _call(dev, "selective_scan_prefill", lib.selective_scan_prefill, _p(x), xs, _p(dt), dts, dt.dtype == torch.bfloat16,
           _p(A), _p(B), bs, _p(C), cs, _p(D), _p(dt_bias), bool(dt_softplus), _p(s0), _p(y), _p(sf), _p(cu), n, T, H, P,

@@ -10,7 +10,7 @@ import torch
 
 from conftest import ROOT
 import gdn_b200
-from gdn_b200 import _lib
+from gdn_b200 import _lib, ssm
 from gdn_b200.ssm import _rows
 
 INVALID = 1  # cudaErrorInvalidValue
@@ -129,3 +129,38 @@ def test_rows_keeps_slices_and_copies_the_rest():
     assert s == 8 and t.data_ptr() % 16 == 0
     t, s = _rows(torch.zeros(2, 0, 8), 2)
     assert s >= 8
+
+
+def test_every_call_of_a_scan_runs_on_the_inputs_device(monkeypatch):
+    """The scratch is planned for the device that the kernels run on, not for the thread's current one (a fake of
+    the library notes which device is current; CPU tensors stand in, whose device index is -1)."""
+    current, calls = [0], []
+
+    class On:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.dev
+
+        def __exit__(self, *e):
+            current[0] = self.before
+
+    class Lib:
+        def selective_scan_scratch_size(self, *a):
+            calls.append(("size", current[0]))
+            return 512
+
+        def selective_scan_prefill(self, *a):
+            calls.append(("launch", current[0]))
+            return 0
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(ssm, "_raw_stream", lambda dev: 0)
+    monkeypatch.setattr(ssm, "_on_one_device", lambda *t: -1)
+    monkeypatch.setattr(ssm, "_status", lambda dev: 0)
+    monkeypatch.setattr(ssm, "load_library", Lib)
+    b = torch.zeros(1, 20, 1, 8, dtype=torch.bfloat16)
+    gdn_b200.selective_scan_prefill(b, torch.zeros(1, 20, 1), torch.zeros(1), b, b)
+    assert calls == [("size", -1), ("launch", -1)] and current == [0]
