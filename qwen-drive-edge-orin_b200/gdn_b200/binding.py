@@ -53,18 +53,21 @@ def _same_device(*ts):
 
 
 _ws_lock = threading.Lock()
+# device index -> its workspaces in the order of their making, each larger than the ones before
 _ws_cache: dict = {}
 
 
 def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
-    """Per-device workspace (status header), zeroed on first use and reused."""
+    """Per-device workspace (status header), zeroed on first use and reused: the first made that is large enough.
+    None is ever replaced or freed: a captured graph or a call in flight may hold its address."""
     key = device.index if device.index is not None else torch.cuda.current_device()
     with _ws_lock:
-        ws = _ws_cache.get(key)
-        if ws is None or ws.numel() < nbytes:
-            ws = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device)
-            _ws_cache[key] = ws
-        return ws
+        made = _ws_cache.setdefault(key, [])
+        for ws in made:
+            if ws.numel() >= nbytes:
+                return ws
+        made.append(torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device))
+        return made[-1]
 
 
 def workspace_size(B: int, T: int, HV: int, debug: bool = False) -> int:
@@ -74,14 +77,18 @@ def workspace_size(B: int, T: int, HV: int, debug: bool = False) -> int:
 
 
 def read_status(device=None, clear: bool = True) -> int:
-    """Device status word of the cached workspace (0 = clean; bit 0 = a bounded wait timed out)."""
+    """Device status word of the cached workspaces, all of the device's together (0 = clean; bit 0 = a bounded
+    wait timed out)."""
     lib = load_library()
     dev = torch.device("cuda", torch.cuda.current_device() if device is None else device)
-    ws = _workspace(dev, 256)
-    out = ctypes.c_int(0)
+    _workspace(dev, 256)
+    status = 0
     with torch.cuda.device(dev):
-        _check(lib.deltanet_read_status(_ptr(ws), ctypes.byref(out), int(clear), _stream()), "deltanet_read_status")
-    return out.value
+        for ws in list(_ws_cache[dev.index]):
+            out = ctypes.c_int(0)
+            _check(lib.deltanet_read_status(_ptr(ws), ctypes.byref(out), int(clear), _stream()), "deltanet_read_status")
+            status |= out.value
+    return status
 
 
 def _check_inputs(q, k, v, g, beta, varlen=False):

@@ -61,11 +61,9 @@ def _on_one_device(first, *others):
 
 
 def _status(dev):
-    """Address of the status word of the device's cached workspace (the one ``read_status`` reads)."""
-    ws = _ws_cache.get(dev)
-    if ws is None:
-        ws = _workspace(torch.device("cuda", dev), 256)
-    return ws.data_ptr()
+    """Address of the status word of the device's first cached workspace (one of those that ``read_status`` reads)."""
+    made = _ws_cache.get(dev)
+    return (made[0] if made else _workspace(torch.device("cuda", dev), 256)).data_ptr()
 
 
 def _rows(t, lead, align=1):

@@ -10,7 +10,7 @@ import torch
 
 from conftest import ROOT
 import gdn_b200
-from gdn_b200 import _lib, ssm
+from gdn_b200 import _lib, binding, ssm
 from gdn_b200.ssm import _rows
 
 INVALID = 1  # cudaErrorInvalidValue
@@ -164,3 +164,44 @@ def test_every_call_of_a_scan_runs_on_the_inputs_device(monkeypatch):
     b = torch.zeros(1, 20, 1, 8, dtype=torch.bfloat16)
     gdn_b200.selective_scan_prefill(b, torch.zeros(1, 20, 1), torch.zeros(1), b, b)
     assert calls == [("size", -1), ("launch", -1)] and current == [0]
+
+
+def test_a_workspace_is_never_replaced(monkeypatch):
+    """A captured graph holds the address of the workspace it was captured with: a larger one later leaves it alive,
+    the small calls keep using it, and its status word is still read (and cleared) with the larger one's."""
+    cache = {}
+    monkeypatch.setattr(binding, "_ws_cache", cache)
+    monkeypatch.setattr(ssm, "_ws_cache", cache)
+    cpu = torch.device("cpu", 0)
+    small = binding._workspace(cpu, 256)
+    large = binding._workspace(cpu, 4096)
+    assert large.numel() >= 4096 and not large.any()
+    assert binding._workspace(cpu, 256).data_ptr() == small.data_ptr() == ssm._status(0)
+    assert binding._workspace(cpu, 3000).data_ptr() == large.data_ptr()
+
+    class Lib:
+        @staticmethod
+        def deltanet_read_status(ws, out, clear, stream):
+            word = ctypes.cast(ws, ctypes.POINTER(ctypes.c_int))
+            out._obj.value = word[0]
+            if clear:
+                word[0] = 0
+            return 0
+
+    class On:
+        def __init__(self, dev):
+            pass
+
+        def __enter__(self):
+            pass
+
+        def __exit__(self, *e):
+            pass
+
+    monkeypatch.setattr(binding, "load_library", Lib)
+    monkeypatch.setattr(binding, "_stream", lambda: None)
+    monkeypatch.setattr(torch.cuda, "device", On)
+    small.view(torch.int32)[0], large.view(torch.int32)[0] = 1 | 1 << 16, 1 | 1 << 15
+    assert binding.read_status(0, clear=False) == 1 | 1 << 15 | 1 << 16
+    assert binding.read_status(0) == 1 | 1 << 15 | 1 << 16
+    assert binding.read_status(0) == 0
