@@ -21,7 +21,11 @@
 // Precision. G and all sums are fp32. M and the state operand of C S^T are rounded to bf16 once (y is
 // a bf16 output, and each of its terms is off by at most one more rounding of that size). The state itself is an fp32 output and carries
 // over thousands of tokens: X' is split exactly into three bf16 terms (8 + 8 + 8 bits of an fp32 value),
-// so its products are those of fp32 operands.
+// so its products are those of fp32 operands; and as the tensor cores truncate their fp32 sums, they only sum
+// what is of a chunk's size (output pass: the chunk's sum and the state's remainder beside its bf16 copy; state
+// pass: up to four chunks), which joins the rest in rounded fp32 additions. Final states of 65536 tokens of one
+// sign with almost no decay are off by 4e-6 of their value in one pass and 6e-6 in segments (7.6e-4 and 4.3e-5 with the whole
+// state as the accumulator; the steps that mend it cost 4%: 8 x 4096 x 64 heads 270 -> 283 us).
 //
 // Decays are kept as base-2 logarithms, relative to 32-token blocks: e^{c_i - c_j} is a row factor times
 // a column factor, one exponential per row and block. Across blocks both are at most 1; inside a block
@@ -100,6 +104,8 @@ constexpr uint32_t TM_Y = 128;   // y fp32 [token][slot, channel]
 constexpr uint32_t TM_S = 256;   // S fp32 [slot, channel][state]
 constexpr uint32_t TM_X = 384;   // X'^T bf16 pairs [slot, channel][token]: 2 pieces x 3 terms x 16 columns
 constexpr uint32_t TM_XP = 48;   // columns per piece
+// (state pass: pieces from column 0 on, two accumulators at TM_S and TM_S + 128)
+constexpr int GROUP = 4;         // chunks that a state pass accumulates in TMEM before it adds them to its sum
 
 // Barriers. *F full, *E empty. A phase is waited for by its parity, so a waiter may neither skip a
 // phase nor let two complete before it looks: every waiter below waits for each phase of its barrier
@@ -175,7 +181,11 @@ __device__ __forceinline__ void scale32(uint32_t (&r)[32], uint64_t f) {
         r[j + 1] = __float_as_uint(x1);
     }
 }
-__device__ __forceinline__ uint32_t pack_bits(uint32_t a, uint32_t b) { return pack_bf16(__uint_as_float(a), __uint_as_float(b)); }
+// A bf16 pair as two fp32 values, by the byte selector of its first half, or zeros.
+constexpr uint32_t HALF_VALUE = 0x1044, HALF_ZERO = 0x4444;
+__device__ __forceinline__ uint64_t halves(uint32_t u, uint32_t first) {
+    return f2_pack(__uint_as_float(__byte_perm(u, 0, first)), __uint_as_float(__byte_perm(u, 0, first + 0x2200)));
+}
 // Address of a row of a 1024-aligned swizzled panel; its 16-byte chunk c is at that address ^ (c << 4).
 __device__ __forceinline__ uint32_t row_at(uint32_t panel, int row) { return panel + row * 128 + ((row & 7) << 4); }
 // Makes a value opaque here, so that what is derived from it is formed in place and not kept in
@@ -211,6 +221,7 @@ __device__ __forceinline__ float4 lds4(uint32_t addr) {
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
     return v;
 }
+__device__ __forceinline__ float4 add4(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
 __device__ __forceinline__ void sts1(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 __device__ __forceinline__ void sts4(uint32_t addr, float4 v) {
     asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
@@ -304,8 +315,9 @@ __device__ __forceinline__ void find_segment(const ScanArgs& a, int seg_tokens, 
 
 // kState: the state pass of a segmented call: every segment but a sequence's last from a zero state. With
 // weights that decay to the segment's end (chunks in reverse order, the later chunks' decay carried along)
-// the state is one long product: no decay of the state, no chain between chunks, four pieces in flight;
-// its final state and log decay go to part / part_log, no output.
+// the state is one long product: no decay of the state, no chain between chunks, four pieces in flight. Groups
+// of GROUP chunks take turns in two accumulators; warps 8-15 add each finished one to a sum in shared memory.
+// The segment's final state and log decay go to part / part_log, no output.
 template <bool kState>
 __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __grid_constant__ ChunkParams p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -403,6 +415,10 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
     auto sums = [&](int buf, int s) { return sb + OFF_MISC + MISC_SUMS + (uint32_t)(2 * buf + s) * 16; };
     auto exps = [&](int buf, int s) { return sb + OFF_MISC + MISC_EXP + (uint32_t)(2 * buf + s) * 4; };
     const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16);  // this warp's TMEM lane quarter
+    // State pass, group g of its chunks: accumulated (each accumulator has barriers of its own, so that no phase
+    // of one can pass unseen behind the other's) and read by the warps that add it up.
+    auto sum_done = [](int g) { return g & 1 ? B_YD : B_SD; };
+    auto sum_read = [](int g) { return g & 1 ? B_MR : B_SC; };
 
     // ---- X'^T (warps 0-15): warpgroup i forms piece i of a chunk, 32 tokens; a thread one slot channel
     // (TMEM lane), whose tokens it reads down a column of the x tile (64 contiguous bytes a warp).
@@ -469,6 +485,15 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
         const bool second_half = warp >= 8;
         const int cols = wg & 1;  // y: slot; state: 64-column panel
         const uint32_t tm_s = tl + TM_S + 64 * cols, tm_y = tl + TM_Y + 64 * cols;
+        // S = decay x (its bf16 copy in shared memory) + (TMEM): see the state's step below
+        float decay = 0.f;
+        uint32_t half = HALF_VALUE;
+        auto copy_row = [&]() {
+            uint32_t at = row_at(sb + OFF_S + cols * PANEL, row);
+            keep_local(at);
+            return at;
+        };
+        const uint32_t kept = sb + (cols ? OFF_S : OFF_C) + 16 * row;  // state pass: the sum, [state / 4][row] of this panel
         float D = 0.f;
         if (!kState && second_half && a.D != nullptr) D = a.D[slot_head(cols)];
         if (!kState && second_half && !idle) {  // entry state: the initial state, or the one that scan_entry_kernel left
@@ -477,15 +502,21 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
             if (later) ptx::grid_dependency_wait();
             const size_t sbase = (((size_t)seg[SEG_SEQ] * a.H + slot_head(s)) * a.P + ch) * a.NS + 64 * cols;
             const bool inside = !kState && a.s0 != nullptr && ch < a.P;
+            const uint32_t copy = copy_row();
+            bool wild = false;
 #pragma unroll 1
             for (int q4 = 0; q4 < 4; ++q4) {
                 float v[16];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (later) f = p.part[((size_t)blockIdx.x * 32 + 16 * cols + 4 * q4 + c) * CH + row];
-                    else if (inside && 64 * cols + 16 * q4 + 4 * c < a.NS) f = *reinterpret_cast<const float4*>(a.s0 + sbase + 16 * q4 + 4 * c);
+                    if (64 * cols + 16 * q4 + 4 * c < a.NS) {
+                        if (later) f = p.part[((size_t)blockIdx.x * 32 + 16 * cols + 4 * q4 + c) * CH + row];
+                        else if (inside) f = *reinterpret_cast<const float4*>(a.s0 + sbase + 16 * q4 + 4 * c);
+                    }
                     v[4 * c] = f.x, v[4 * c + 1] = f.y, v[4 * c + 2] = f.z, v[4 * c + 3] = f.w;
+                    wild |= !(fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w))) < 3.38e38f);
+                    if (c & 1) st_shared_v4(copy ^ ((2 * q4 + (c >> 1)) << 4), 0, 0, 0, 0);
                 }
                 uint32_t o[16];
 #pragma unroll
@@ -493,6 +524,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 ptx::tmem_st16(tm_s + 16 * q4, o);
             }
             ptx::tmem_wait_st();
+            // infinities (and what bf16 rounds to them) have no remainder: such a state stays whole in TMEM
+            if (__any_sync(0xffffffffu, wild)) half = HALF_ZERO;
         }
         auto output = [&](int k) {  // y = Y + D x, in place of x
             const int buf = k & 1, valid = min(CH, len - CH * k), s = cols;
@@ -555,9 +588,29 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                     ptx::mbar_arrive(bar(B_PE + buf));
                     ptx::mbar_arrive(bar(B_XE + buf));
                 }
+                if (second_half && k > 0 && k % GROUP == 0) {  // the group before this chunk's, onto the sum
+                    const int g = k / GROUP - 1;
+                    team_wait([&] { wait(sum_done(g), (uint32_t)g >> 1); });
+                    ptx::tc_fence_after();
+#pragma unroll 1
+                    for (int q4 = 0; q4 < 4; ++q4) {
+                        float v[16];
+                        ptx::tmem_ld16(tm_s + 128 * (g & 1) + 16 * q4, v);
+                        ptx::tmem_wait_ld();
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const uint32_t at = kept + (4 * q4 + c) * (CH * 16);
+                            float4 f = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+                            if (g > 0) f = add4(f, lds4(at));
+                            sts4(at, f);
+                        }
+                    }
+                    ptx::tc_fence_before();
+                    warp_arrive(sum_read(g));
+                }
             }
             if (second_half && nc > 0) {
-                team_wait([&] { wait(B_SD, 0); });
+                team_wait([&] { wait(sum_done((nc - 1) / GROUP), (uint32_t)((nc - 1) / GROUP) >> 1); });
                 ptx::tc_fence_after();
             }
         } else {
@@ -567,7 +620,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
             if (second_half) {
                 const int valid = min(CH, len - CH * k);
                 if (k < nc) {
-                    // the state: bf16 copy as the operand of C S^T, and its decay over this chunk
+                    // The state S: a bf16 copy as the operand of C S^T, and the decay of the rest over this chunk.
+                    // The tensor cores cut off the bits of a sum below its last place, 24 times a chunk: with
+                    // the whole state as the accumulator its error grew by 1.5e-6 of it a chunk, all one way
+                    // (7.6e-4 after 65536 tokens of inputs of one sign). So TMEM holds only what the copy's
+                    // rounding left out, and takes the chunk's sum onto that; S is put together again here, in
+                    // fp32 with one rounding.
                     team_wait([&] {
                         wait(B_PF + buf, (uint32_t)k >> 1);
                         if (k > 0) wait(B_SD, k - 1);
@@ -577,22 +635,31 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                     if (cols < npanel) {
                         const float4 R = lds4(sums(buf, quarter >> 1));
                         const float total = (R.x + R.y) + (R.z + R.w);
-                        const float decay = ex2f(total);
+                        const uint64_t before = f2_pack(decay, decay);
+                        decay = ex2f(total);
                         const uint64_t dd = f2_pack(decay, decay);
 #pragma unroll 1
                         for (int hf = 0; hf < 2; ++hf) {
                             uint32_t v[32];
                             tmem_ld32u(tm_s + 32 * hf, v);
                             ptx::tmem_wait_ld();
-                            {
-                                uint32_t at = row_at(sb + OFF_S + cols * PANEL, row);
-                                keep_local(at);
+                            const uint32_t at = copy_row();
 #pragma unroll
-                                for (int c = 0; c < 4; ++c)
-                                    st_shared_v4(at ^ ((4 * hf + c) << 4), pack_bits(v[8 * c], v[8 * c + 1]), pack_bits(v[8 * c + 2], v[8 * c + 3]),
-                                                 pack_bits(v[8 * c + 4], v[8 * c + 5]), pack_bits(v[8 * c + 6], v[8 * c + 7]));
+                            for (int c = 0; c < 4; ++c) {
+                                uint32_t u[4];
+                                ld_shared_v4(at ^ ((4 * hf + c) << 4), u[0], u[1], u[2], u[3]);
+#pragma unroll
+                                for (int t = 0; t < 4; ++t) {
+                                    uint32_t &v0 = v[8 * c + 2 * t], &v1 = v[8 * c + 2 * t + 1];
+                                    const uint64_t S = f2_fma(halves(u[t], half), before, f2_pack(__uint_as_float(v0), __uint_as_float(v1)));
+                                    float x0, x1;
+                                    f2_unpack(S, x0, x1);
+                                    u[t] = pack_bf16(x0, x1);
+                                    f2_unpack(f2_mul(f2_sub(S, halves(u[t], half)), dd), x0, x1);
+                                    v0 = __float_as_uint(x0), v1 = __float_as_uint(x1);
+                                }
+                                st_shared_v4(at ^ ((4 * hf + c) << 4), u[0], u[1], u[2], u[3]);
                             }
-                            scale32(v, dd);
                             ptx::tmem_st32(tm_s + 32 * hf, v);
                         }
                         ptx::tmem_wait_st();
@@ -700,17 +767,27 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
         }
         }
         if (second_half && !idle && (kState || seg[SEG_J] == seg[SEG_COUNT] - 1)) {
+            const int last = kState ? (nc - 1) / GROUP : 0;
+            const uint64_t before = f2_pack(decay, decay);
+            const uint32_t copy = copy_row();
             const int s = quarter >> 1, ch = slot_tile(s) + (row & 63);
             const size_t sbase = (((size_t)seg[SEG_SEQ] * a.H + slot_head(s)) * a.P + ch) * a.NS + 64 * cols;
             const bool inside = ch < a.P && (s == 0 || seg[SEG_SECOND]);
 #pragma unroll 1
             for (int q4 = 0; q4 < 4; ++q4) {
                 float v[16];
-                ptx::tmem_ld16(tm_s + 16 * q4, v);
+                ptx::tmem_ld16(tm_s + 128 * (last & 1) + 16 * q4, v);
                 ptx::tmem_wait_ld();
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const float4 f = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+                    float4 f = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+                    if (kState) {
+                        if (last > 0) f = add4(f, lds4(kept + (4 * q4 + c) * (CH * 16)));
+                    } else {
+                        const uint32_t at = (copy ^ ((2 * q4 + (c >> 1)) << 4)) + 8 * (c & 1);
+                        f2_unpack(f2_fma(halves(__float_as_uint(lds1(at)), half), before, f2_pack(f.x, f.y)), f.x, f.y);
+                        f2_unpack(f2_fma(halves(__float_as_uint(lds1(at + 4)), half), before, f2_pack(f.z, f.w)), f.z, f.w);
+                    }
                     if (kState)
                         p.part[((size_t)blockIdx.x * 32 + 16 * cols + 4 * q4 + c) * CH + row] = f;
                     else if (inside && 64 * cols + 16 * q4 + 4 * c < a.NS)
@@ -740,6 +817,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 for (int k = 0; k < nc; ++k) {
                     wait(B_BF + (k & 1), (uint32_t)k >> 1);
                     if (!kState) wait(B_SC, k);
+                    const int g = kState ? k / GROUP : 0;
+                    if (kState && k % GROUP == 0 && g >= 2) wait(sum_read(g), (uint32_t)(g - 2) >> 1);
 #pragma unroll 1
                     for (int i = 0; i < PIECES; ++i) {
                         wait(B_RF + i, k);
@@ -749,14 +828,14 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                         for (int st = 0; st < PIECE / 16; ++st)
 #pragma unroll
                             for (int term = 0; term < 3; ++term)
-                                ptx::mma_bf16_ts(tmem + TM_S,
+                                ptx::mma_bf16_ts(tmem + TM_S + 128 * (g & 1),
                                                  tmem + (kState ? TM_G + TM_XP * i : TM_X + TM_XP * (i & 1)) + 16 * term + 8 * st,
                                                  desc(dpanel, b_off(k) + (uint32_t)(PIECE * i + 16 * st) * 128u), id_state,
-                                                 !kState || k + i + st + term > 0);
+                                                 !kState || k % GROUP + i + st + term > 0);
                         ptx::mma_commit(bar(B_RE + i));
                     }
                     if (dead) break;
-                    if (!kState || k == nc - 1) ptx::mma_commit(bar(B_SD));
+                    if (kState ? k % GROUP == GROUP - 1 || k == nc - 1 : true) ptx::mma_commit(bar(kState ? sum_done(g) : B_SD));
                     ptx::mma_commit(bar(B_BE + (k & 1)));
                 }
             } else if (!kState) {

@@ -239,6 +239,47 @@ def test_scan_segments_of_long_sequences(n, T, H, P, G, N):
         check_scan(y[i], sf[i], scan_ref(s["x"][i], s["dt"][i], s["A"], s["B"][i], s["C"][i], s["D"], s["dt_bias"], s0[i]))
 
 
+@pytest.mark.parametrize("n,T,H,P,G,N,cut", [(10, 32768, 64, 8, 1, 8, False), (5, 16384, 64, 64, 1, 72, True), (1, 65536, 2, 64, 1, 16, True),
+                                             (1, 65536, 4, 72, 2, 128, True)])
+@pytest.mark.parametrize("A", [-1e-6, -0.01])
+def test_scan_state_of_long_prompts_does_not_drift(n, T, H, P, G, N, cut, A):
+    """Inputs of one sign and almost no decay: the state is a sum of tens of thousands of terms, none of which cancel.
+    Bound, relative to the state. The tensor cores cut off each partial sum of a chunk's 24 products below its last
+    place (2^-23 of it): over a group of g chunks that start from zero, half of 24 g 2^-23, with g <= 4 5.7e-6. The
+    chunks' sums join by at most 512 rounded additions, whose errors (2^-24 each, both ways) add up to 4 sqrt(512) 2^-24 =
+    5.4e-6 at four standard deviations and more. Decays: logarithms up to some 30, whose fp32 sums are off by a few
+    2^-24 of them: 6e-6. In all 2e-5."""
+    assert segmented(n, T, False, H, P, G, N) == cut
+    g = gen(T + N)
+    s = scan_inputs(g, (n, T), H, P, G, N, bias=False, D=False)
+    s["x"], s["B"], s["dt"] = s["x"].abs(), s["B"].abs(), 0.01 + 0.1 * s["dt"].abs()
+    s["A"] = torch.full((H,), A, device=DEV)
+    s0 = nrm(g, n, H, P, N).abs()
+    _, sf = gdn_b200.selective_scan_prefill(**s, s0=s0)
+    for i in {0, n - 1}:
+        c = (s["dt"][i].double() * A).cumsum(0)
+        w = torch.exp(c[-1] - c) * s["dt"][i].double()
+        for h in (0, H - 1):
+            S = (s["x"][i, :, h].double() * w[:, h, None]).T @ s["B"][i, :, h * G // H].double() + torch.exp(c[-1, h]) * s0[i, h].double()
+            close(sf[i, h], S, 2e-5 * S)
+
+
+@pytest.mark.parametrize("T", [130, 3000])
+def test_scan_keeps_an_infinite_initial_state(T):
+    """Infinities in the initial state stay where they are, with their sign; the rest of the state is as without them."""
+    g = gen(T)
+    s = scan_inputs(g, (1, T), 2, 64, 1, 128)
+    s["A"] = -torch.full((2,), 1e-3, device=DEV)
+    s0 = nrm(g, 1, 2, 64, 128)
+    _, want = gdn_b200.selective_scan_prefill(**s, s0=s0, dt_softplus=True)
+    s0[0, 0, 3, 5], s0[0, 1, 40, 100] = math.inf, -math.inf
+    _, sf = gdn_b200.selective_scan_prefill(**s, s0=s0, dt_softplus=True)
+    assert sf[0, 0, 3, 5] == math.inf and sf[0, 1, 40, 100] == -math.inf
+    ok = torch.isfinite(s0)
+    # (the two ways of accumulating differ by the hardware's truncation: 24 steps of 2^-23 a chunk)
+    assert ((sf - want).abs()[ok] <= 24 * 24 * 2.0 ** -23 * want[ok].abs().max()).all()
+
+
 def test_scan_segments_of_a_packed_batch():
     """Segments of sequences of unlike lengths, empty ones among them, NaN behind the last."""
     lens, H, P, G, N = [900, 0, 1, 128, 1700, 257, 0], 2, 64, 1, 64
