@@ -234,7 +234,7 @@ cudaError_t deltanet_noalloc_read_status(int* status_host, int clear, cudaStream
  * after about 1 s). The bits above say which part gave up: 8-11 the
  * cluster-split kernel's chain CTA (compute warps, MMA warp, load warp, output
  * MMA warp), 12-13 its prep CTAs (compute warps, gate warp), 14 its output CTA,
- * 15 the one-CTA-per-head kernel. Clears it when clear != 0. No counterpart in
+ * 15 the one-CTA-per-head kernel, 16 the selective scan (gdn_ssm.h). Clears it when clear != 0. No counterpart in
  * the reference (its kernels have no waits). */
 cudaError_t deltanet_read_status(void* workspace, int* status_host, int clear, cudaStream_t stream);
 

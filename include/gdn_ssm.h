@@ -66,6 +66,15 @@ cudaError_t selective_scan_prefill(const void* x, int64_t x_stride, const void* 
                                    void* workspace, size_t workspace_bytes, void* scratch, size_t scratch_bytes,
                                    cudaStream_t stream);
 
+/* Test hook for failure detection: selective_scan_prefill of N sequences of T tokens (at least 16; contiguous
+ * inputs, fp32 dt, no D, dt_bias, softplus or s0) with the x tiles of chunk `withheld_chunk` (of 128 tokens, counted in
+ * each segment) never loaded. The waits for them run out, the status word says so, the kernels stop, wait (bounded)
+ * for what they have in flight and return; y and sf are then undefined. Returns the launch status. */
+cudaError_t selective_scan_test_withheld_load(const void* x, const void* dt, const float* A, const void* B,
+                                              const void* C, void* y, float* sf, int N, int T, int H, int P, int G,
+                                              int n_state, void* workspace, size_t workspace_bytes, void* scratch,
+                                              size_t scratch_bytes, cudaStream_t stream, int withheld_chunk);
+
 /* The next T tokens (usually one) of `N` sequences, x [N, T, H, P], with the state [N, H, P, N_STATE]
  * read and updated in place. Continues a prefill from its final state. */
 cudaError_t selective_scan_decode(const void* x, int64_t x_stride, const void* dt, int64_t dt_stride, int dt_bf16,

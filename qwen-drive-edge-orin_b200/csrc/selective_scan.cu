@@ -38,6 +38,21 @@ static bool scan_args_ok(const ScanArgs& a, int64_t rows) {
     return aligned_to(a.x, 16) && aligned_to(a.B, 16) && aligned_to(a.C, 16) && aligned_to(a.y, 16);
 }
 
+// withhold: see launch_scan_chunks; such a call never runs token by token.
+static cudaError_t scan_prefill(const ScanArgs& a, void* workspace, size_t workspace_bytes, void* scratch, size_t scratch_bytes,
+                                int withhold, cudaStream_t stream) {
+    const int64_t rows = a.cu ? a.T : (int64_t)a.N * a.T;
+    if (!scan_args_ok(a, rows)) return cudaErrorInvalidValue;
+    if (!workspace || workspace_bytes < 256) return cudaErrorInvalidValue;
+    if (a.N == 0) return cudaSuccess;
+    if (a.T <= STEP_TOKENS) return withhold < 0 ? launch_scan_step(a, stream) : cudaErrorInvalidValue;
+    if (rows > 0x7fffffffLL - 128) return cudaErrorInvalidValue;  // token rows are 32-bit tile coordinates
+    const ChunkPlan pl = plan_scan_chunks(a.N, a.T, a.cu != nullptr, a.H, a.P, a.G, sm_count());
+    if (pl.part_bytes > 0 && (!scratch || !aligned_to(scratch, 256) || scratch_bytes < pl.log_bytes + pl.part_bytes))
+        return cudaErrorInvalidValue;
+    return launch_scan_chunks(a, pl, rows, workspace, scratch, withhold, stream);
+}
+
 }  // namespace ssm
 }  // namespace gdn
 
@@ -59,17 +74,22 @@ extern "C" cudaError_t selective_scan_prefill(const void* x, int64_t x_stride, c
     gdn::ssm::ScanArgs a{static_cast<const bf16*>(x), static_cast<const bf16*>(B), static_cast<const bf16*>(C), dt, A, D,
                          dt_bias, s0, sf, static_cast<bf16*>(y), cu_seqlens, x_stride, dt_stride, B_stride, C_stride, N, T,
                          H, P, G, n_state, dt_bf16, dt_softplus};
-    const int64_t rows = cu_seqlens ? T : (int64_t)N * T;
-    if (!gdn::ssm::scan_args_ok(a, rows)) return cudaErrorInvalidValue;
-    if (!workspace || workspace_bytes < 256) return cudaErrorInvalidValue;
-    if (N == 0) return cudaSuccess;
-    if (T <= gdn::ssm::STEP_TOKENS) return gdn::ssm::launch_scan_step(a, stream);
-    if (rows > 0x7fffffffLL - 128) return cudaErrorInvalidValue;  // token rows are 32-bit tile coordinates
-    const gdn::ssm::ChunkPlan pl =
-        gdn::ssm::plan_scan_chunks(N, T, cu_seqlens != nullptr, H, P, G, gdn::ssm::sm_count());
-    if (pl.part_bytes > 0 && (!scratch || !gdn::aligned_to(scratch, 256) || scratch_bytes < pl.log_bytes + pl.part_bytes))
-        return cudaErrorInvalidValue;
-    return gdn::ssm::launch_scan_chunks(a, pl, rows, workspace, scratch, stream);
+    return gdn::ssm::scan_prefill(a, workspace, workspace_bytes, scratch, scratch_bytes, -1, stream);
+}
+
+// Test hook for the bounded waits: the x tiles of one chunk never arrive, so that the waits for them run out.
+// No fault, trap or unbounded wait is involved.
+extern "C" cudaError_t selective_scan_test_withheld_load(const void* x, const void* dt, const float* A, const void* B,
+                                                         const void* C, void* y, float* sf, int N, int T, int H, int P,
+                                                         int G, int n_state, void* workspace, size_t workspace_bytes,
+                                                         void* scratch, size_t scratch_bytes, cudaStream_t stream,
+                                                         int withheld_chunk) {
+    using bf16 = __nv_bfloat16;
+    if (withheld_chunk < 0) return cudaErrorInvalidValue;
+    gdn::ssm::ScanArgs a{static_cast<const bf16*>(x), static_cast<const bf16*>(B), static_cast<const bf16*>(C), dt, A, nullptr,
+                         nullptr, nullptr, sf, static_cast<bf16*>(y), nullptr, (int64_t)H * P, H, (int64_t)G * n_state,
+                         (int64_t)G * n_state, N, T, H, P, G, n_state, 0, 0};
+    return gdn::ssm::scan_prefill(a, workspace, workspace_bytes, scratch, scratch_bytes, withheld_chunk, stream);
 }
 
 extern "C" cudaError_t selective_scan_decode(const void* x, int64_t x_stride, const void* dt, int64_t dt_stride,

@@ -34,8 +34,9 @@ struct ChunkPlan {
     size_t part_bytes, log_bytes;
 };
 ChunkPlan plan_scan_chunks(int N, int T, bool packed, int H, int P, int G, int sms);
+// withhold: test hook, the chunk of each segment whose x tiles are never loaded (-1: none).
 cudaError_t launch_scan_chunks(const ScanArgs& a, const ChunkPlan& pl, int64_t rows, void* workspace, void* scratch,
-                               cudaStream_t stream);
+                               int withhold, cudaStream_t stream);
 
 // Step size of (row, head) before the bias and the softplus.
 __device__ __forceinline__ float scan_dt(const ScanArgs& a, int64_t row, int h) {

@@ -142,6 +142,7 @@ struct ChunkParams {
     int units;         // G * pairs
     int seg_tokens;    // tokens per segment (a multiple of 128), 0: one segment per sequence
     int segments;      // segments that part and part_log have room for
+    int withhold;      // test hook: chunk of each segment whose x tiles are never loaded (-1: none)
 };
 
 // The rest of a wait whose first test failed, out of line (the kernel has some thirty waits and is
@@ -897,7 +898,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
             if (!kState) ptx::prefetch_tensormap(&p.tm_c);
             const int h0 = slot_head(0), h1 = slot_head(1), t0 = slot_tile(0), t1 = slot_tile(1), row0 = seg[SEG_ROW], g = seg[SEG_GROUP];
             const bool second = seg[SEG_SECOND];
-            int nb = 0, nx = 0, ncl = 0;  // loads issued
+            int nb = 0, nx = 0, ncl = 0;  // loads issued (nx: up to this chunk)
             auto load_b = [&](int k) {
                 if (dead || k >= nc) return;
                 ++nb;
@@ -914,8 +915,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 for (int c = 0; c < npanel; ++c) ptx::tma_load_4d(sb + OFF_C + c * PANEL, &p.tm_c, bar(B_CF), 64 * c, g, row0 + CH * k, 0);
             };
             auto load_x = [&](int k) {
-                if (dead || k >= nc) return;
-                ++nx;
+                if (dead || k >= nc || k == p.withhold) return;
+                nx = k + 1;
                 const int buf = k & 1;
                 ptx::mbar_arrive_expect_tx(bar(B_XF + buf), 2 * PANEL);
                 ptx::tma_load_4d(sb + OFF_X + 2 * buf * PANEL, &p.tm_x, bar(B_XF + buf), t0, h0, chunk_row(row0, k), 0);
@@ -951,15 +952,16 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) scan_chunk_kernel(const __gr
                 }
             }
             // nothing in flight when the CTA leaves
-            const bool failed = dead;
-            dead = false;
+            auto landed = [&](int b, uint32_t parity) {  // (each wait by itself, whatever ran out before)
+                dead = false;
+                wait(b, parity);
+            };
             for (int buf = 0; buf < 2; ++buf) {
-                if (nb > buf) wait(B_BF + buf, (uint32_t)(nb - 1 - buf) >> 1);
-                if (nx > buf) wait(B_XF + buf, (uint32_t)(nx - 1 - buf) >> 1);
+                if (nb > buf) landed(B_BF + buf, (uint32_t)(nb - 1 - buf) >> 1);
+                if (nx > buf) landed(B_XF + buf, (uint32_t)(nx - 1 - buf) >> 1);
             }
-            if (ncl > 0) wait(B_CF, (uint32_t)(ncl - 1));
+            if (ncl > 0) landed(B_CF, (uint32_t)(ncl - 1));
             ptx::bulk_wait_all();
-            dead |= failed;
         }
         __syncwarp();
     } else if (warp == 18) {
@@ -1220,7 +1222,7 @@ ChunkPlan plan_scan_chunks(int N, int T, bool packed, int H, int P, int G, int s
 }
 
 cudaError_t launch_scan_chunks(const ScanArgs& a, const ChunkPlan& pl, int64_t rows, void* workspace, void* scratch,
-                               cudaStream_t stream) {
+                               int withhold, cudaStream_t stream) {
     ChunkParams p;
     memset(&p, 0, sizeof(p));
     if (!row_map(&p.tm_x, a.x, a.P, a.H, rows, a.xs) || !row_map(&p.tm_b, a.B, a.NS, a.G, rows, a.bs) ||
@@ -1237,6 +1239,7 @@ cudaError_t launch_scan_chunks(const ScanArgs& a, const ChunkPlan& pl, int64_t r
     p.units = pl.units;
     p.seg_tokens = pl.seg_tokens;
     p.segments = (int)pl.segments;
+    p.withhold = withhold;
     const int64_t ctas = pl.segments * pl.units;
     if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
     if (pl.seg_tokens == 0) {

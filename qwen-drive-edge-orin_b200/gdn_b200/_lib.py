@@ -47,6 +47,8 @@ SIGNATURES = {
     "selective_scan_prefill": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64,
                                        c_void_p, c_int64, c_void_p, c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 6
                                + [c_void_p, c_size_t, c_void_p, c_size_t, c_void_p]),
+    "selective_scan_test_withheld_load": (c_int, [c_void_p] * 7 + [c_int] * 6 + [c_void_p, c_size_t, c_void_p, c_size_t,
+                                                                               c_void_p, c_int]),
     "selective_scan_decode": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64,
                                       c_void_p, c_int64, c_void_p, c_void_p, c_int] + [c_void_p] * 2 + [c_int] * 6
                               + [c_void_p]),

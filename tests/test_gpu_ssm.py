@@ -7,6 +7,7 @@ the terms' magnitudes. Each check states its bound from those two.
 from __future__ import annotations
 
 import math
+import time
 
 import pytest
 import torch
@@ -672,3 +673,33 @@ def test_streams_run_side_by_side():
     for i in range(2):
         for y, sf in got[i]:
             assert torch.equal(y, want[i][0]) and torch.equal(sf, want[i][1])
+
+
+@pytest.mark.parametrize("T,cut", [(700, False), (20000, True)])
+def test_scan_withheld_load_times_out_and_the_next_call_is_clean(T, cut):
+    """Failure detection without a fault: tiles that never arrive. The bounded waits (about 1 s each) run out, the
+    status word says so (bit 0, and bit 16 for the scan), the kernels end, and the next call is as before."""
+    n, H, P, G, N = (1, 2, 64, 1, 64) if cut else (4, 40, 64, 1, 64)
+    lib = gdn_b200.load_library()
+    nbytes = lib.selective_scan_scratch_size(n, T, 0, H, P, G, N)
+    assert (nbytes > 0) == cut  # (cut: 53 segments of three chunks)
+    g = gen(T)
+    s = scan_inputs(g, (n, T), H, P, G, N, bias=False, D=False)
+    s["dt"] = s["dt"].abs()
+    want = gdn_b200.selective_scan_prefill(**s)
+    y, sf = torch.empty_like(s["x"]), torch.empty(n, H, P, N, device=DEV)
+    ws, scratch = torch.zeros(64, dtype=torch.int32, device=DEV), torch.empty(max(nbytes, 1), dtype=torch.uint8, device=DEV)
+    torch.cuda.synchronize()
+    start = time.perf_counter()
+    rc = lib.selective_scan_test_withheld_load(s["x"].data_ptr(), s["dt"].data_ptr(), s["A"].data_ptr(), s["B"].data_ptr(), s["C"].data_ptr(),
+                                               y.data_ptr(), sf.data_ptr(), n, T, H, P, G, N, ws.data_ptr(), 256, scratch.data_ptr(),
+                                               nbytes, torch.cuda.current_stream().cuda_stream, 1)
+    assert rc == 0
+    torch.cuda.synchronize()  # raises if a kernel faulted
+    elapsed = time.perf_counter() - start
+    print(f"T={T}: status {int(ws[0]):#x} after {elapsed:.2f} s")
+    assert int(ws[0]) == 1 | 1 << 16 and not ws[1:].any()
+    assert elapsed < 20.0
+    got = gdn_b200.selective_scan_prefill(**s)
+    assert gdn_b200.binding.read_status() == 0
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -205,3 +205,11 @@ def test_a_workspace_is_never_replaced(monkeypatch):
     assert binding.read_status(0, clear=False) == 1 | 1 << 15 | 1 << 16
     assert binding.read_status(0) == 1 | 1 << 15 | 1 << 16
     assert binding.read_status(0) == 0
+
+
+@pytest.mark.parametrize("bad", [dict(T=15), dict(chunk=-1), dict(ws=None), dict(x=None), dict(scrb=0)])
+def test_scan_withheld_load_refuses(bad):
+    a = dict(x=P, dt=P, A=P, B=P, C=P, y=P, sf=P, N=1, T=2000, H=2, P=64, G=1, NS=64, ws=P, wsb=256, scr=P, scrb=1 << 40,
+             stream=None, chunk=1)
+    a.update(bad)
+    assert gdn_b200.load_library().selective_scan_test_withheld_load(*a.values()) == INVALID
