@@ -50,8 +50,8 @@ cudaError_t causal_conv_decode(const void* x, int64_t x_stride, const void* w, c
  * x [rows, H, P], B and C [rows, G, N_STATE] bf16 (heads and groups contiguous inside a row), head h
  * uses group h / (H / G); dt [rows, H] fp32 (dt_bf16 = 0) or bf16 (1); A, D (or NULL), dt_bias (or
  * NULL) fp32 [H]; y bf16 [rows, H, P]; s0 (or NULL: zeros) and sf fp32 [N, H, P, N_STATE].
- * d A <= 0 (a decay). P and N_STATE are multiples of 8 up to 128, N and H at most 65535; x, B, C rows
- * 16-byte aligned. sf must not overlap s0. An x that is not finite makes its
+ * d A <= 0 (a decay). P and N_STATE are multiples of 8 up to 128, N and H at most 65535, token rows at
+ * most 2^31 - 129; x, B, C rows 16-byte aligned. sf must not overlap s0. An x that is not finite makes its
  * channel's outputs NaN from the start of its 128 tokens (counted from the sequence's start) on, not
  * from its own token on; no value of any input reaches another sequence.
  * workspace: at least 256 bytes, zero before its first use, whose first word is the status word

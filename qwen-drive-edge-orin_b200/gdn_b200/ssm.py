@@ -19,6 +19,8 @@ __all__ = ["causal_conv_prefill", "causal_conv_prefill_varlen", "causal_conv_dec
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _MAX_GRID = 65535  # sequences and heads of a scan are grid dimensions
+_MAX_INT = (1 << 31) - 1  # sizes cross the C ABI as int, and ctypes keeps the low bits of larger ones
+_MAX_ROWS = _MAX_INT - 128  # token rows of a scan over prompts (32-bit tile coordinates, whole tiles)
 # the current stream's handle without a Stream object: a single-token call is bound by its host time
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
@@ -161,6 +163,8 @@ def _check_conv(x, w, bias, packed=False):
         raise ValueError("only 2 to 4 taps are supported")
     if C < 1:
         raise ValueError("x needs at least one channel")
+    if B > _MAX_INT or x.shape[1] > _MAX_INT or C > _MAX_INT:
+        raise ValueError("sizes of x must be below 2^31")
     if packed and B != 1:
         raise ValueError("varlen inputs are packed: B must be 1")
     return dev, _vector(bias, C, dtype, "bias", dev)
@@ -242,6 +246,8 @@ def _check_scan(x, dt, A, B, C, D, dt_bias, packed=False):
         raise ValueError("varlen inputs are packed: B must be 1")
     if b > _MAX_GRID or H > _MAX_GRID:
         raise ValueError(f"at most {_MAX_GRID} sequences and heads are supported")
+    if T > _MAX_INT:
+        raise ValueError("sizes must be below 2^31")
     A = _vector(A, H, torch.float32, "A", dev)
     D = _vector(D, H, torch.float32, "D", dev)
     dt_bias = _vector(dt_bias, H, torch.float32, "dt_bias", dev)
@@ -253,6 +259,8 @@ def _scan_prefill(x, dt, A, B, C, D, dt_bias, s0, dt_softplus, cu):
     if cu is not None:
         cu = _offsets(cu, dev)
     n = b if cu is None else cu.numel() - 1
+    if b * T > _MAX_ROWS:
+        raise ValueError(f"at most {_MAX_ROWS} token rows are supported")
     if n > _MAX_GRID:
         raise ValueError(f"at most {_MAX_GRID} sequences and heads are supported")
     s0 = _initial(s0, (n, H, P, N), torch.float32, dev)
@@ -275,8 +283,8 @@ def selective_scan_prefill(x, dt, A, B, C, D=None, dt_bias=None, s0=None, dt_sof
     Per head h of group g = h // (H // G), with d = dt + dt_bias (softplus'ed if ``dt_softplus``):
         S <- exp(d A) S + d x B^T;   y = S C + D x.
     x bf16 [B,T,H,P], dt fp32 or bf16 [B,T,H], B/C bf16 [B,T,G,N], A, D, dt_bias fp32 [H], initial
-    state s0 fp32 [B,H,P,N] or zeros. P and N are multiples of 8 up to 128, B and H at most 65535, and
-    d A <= 0. A token with d = 0 (dt of minus infinity under the softplus) leaves the state as it is, so
+    state s0 fp32 [B,H,P,N] or zeros. P and N are multiples of 8 up to 128, B and H at most 65535, B T at
+    most 2^31 - 129, and d A <= 0. A token with d = 0 (dt of minus infinity under the softplus) leaves the state as it is, so
     padding in front of or between tokens is possible. An x that is not finite
     makes its channel's outputs NaN from the start of its 128 tokens (of its sequence) on.
     """
@@ -323,6 +331,8 @@ def gated_group_rmsnorm(x, z, w, groups: int = 1, eps: float = 1e-6):
     C = x.shape[-1]
     if groups < 1 or C < 1 or C % groups != 0:
         raise ValueError("groups must divide the last dim")
+    if C > _MAX_INT:
+        raise ValueError("the last dim must be below 2^31")
     y = _out(x)
     lead = x.dim() - 1
     (x, xs), (z, zs) = _wide_rows(x, lead, C), _wide_rows(z, lead, C)

@@ -213,3 +213,25 @@ def test_scan_withheld_load_refuses(bad):
              stream=None, chunk=1)
     a.update(bad)
     assert gdn_b200.load_library().selective_scan_test_withheld_load(*a.values()) == INVALID
+
+
+def test_sizes_that_do_not_fit_the_c_abi_are_refused(monkeypatch):
+    """Their low 32 bits would be taken for the size (meta tensors stand in for ones of many GB)."""
+    monkeypatch.setattr(ssm, "_on_one_device", lambda *t: -1)
+    monkeypatch.setattr(ssm, "load_library", lambda: pytest.fail("called the library"))
+    e = lambda *shape, dtype=torch.bfloat16: torch.empty(*shape, dtype=dtype, device="meta")
+    big = (1 << 32) + 5
+    for shape in ((1, big, 1), (big, 1, 1), (1, 1, big)):
+        with pytest.raises(ValueError):
+            gdn_b200.causal_conv_prefill(e(*shape), e(shape[2], 4))
+        with pytest.raises(ValueError):
+            gdn_b200.causal_conv_decode(e(*shape), e(shape[2], 4), e(shape[0], 3, shape[2]))
+    for b, T in ((1, big), (1, (1 << 31) - 128), (65535, 1 << 16)):
+        args = (e(b, T, 1, 8), e(b, T, 1), e(1, dtype=torch.float32), e(b, T, 1, 8), e(b, T, 1, 8))
+        with pytest.raises(ValueError):
+            gdn_b200.selective_scan_prefill(*args)
+        if T == big:
+            with pytest.raises(ValueError):
+                gdn_b200.selective_scan_decode(*args, e(b, 1, 8, 8, dtype=torch.float32))
+    with pytest.raises(ValueError):
+        gdn_b200.gated_group_rmsnorm(e(2, big), e(2, big), e(big))
