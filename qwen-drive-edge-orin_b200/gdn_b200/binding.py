@@ -66,8 +66,26 @@ def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
         for ws in made:
             if ws.numel() >= nbytes:
                 return ws
-        made.append(torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device))
+        made.append(_zeros_now(max(nbytes, 256), device))
         return made[-1]
+
+
+def _zeros_now(nbytes: int, device: torch.device) -> torch.Tensor:
+    """Zeros that are there for every stream when this returns. On a stream of its own: the current one may be
+    capturing a graph, whose replays alone would fill them (each clearing the status again), or be behind other work.
+    The thread's capture mode is relaxed meanwhile, as a capture would refuse the allocation and the wait."""
+    if device.type != "cuda":
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    exchange, mode = load_library().cudaThreadExchangeStreamCaptureMode, ctypes.c_int(2)  # cudaStreamCaptureModeRelaxed
+    side = torch.cuda.Stream(device)
+    _check(exchange(ctypes.byref(mode)), "cudaThreadExchangeStreamCaptureMode")
+    try:
+        with torch.cuda.stream(side):
+            ws = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        side.synchronize()
+    finally:
+        exchange(ctypes.byref(mode))  # (the mode before)
+    return ws
 
 
 def workspace_size(B: int, T: int, HV: int, debug: bool = False) -> int:

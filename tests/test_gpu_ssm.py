@@ -657,6 +657,29 @@ def test_capture_and_replay():
     assert torch.equal(a, b) and torch.equal(ca, cb)
 
 
+def test_capture_of_a_first_call(monkeypatch):
+    """A capture that makes the device's workspace: its status word is zero at once, and replays keep what other calls
+    wrote there."""
+    g = gen(43)
+    s = scan_inputs(g, (1, 200), 2, 64, 1, 64)
+    want = gdn_b200.selective_scan_prefill(**s, dt_softplus=True)  # (loads the kernels)
+    torch.full((1 << 20,), 0x5A, dtype=torch.uint8, device=DEV)  # (freed memory that is not zero)
+    cache = {}
+    monkeypatch.setattr(gdn_b200.binding, "_ws_cache", cache)
+    monkeypatch.setattr(gdn_b200.ssm, "_ws_cache", cache)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = gdn_b200.selective_scan_prefill(**s, dt_softplus=True)
+    (ws,), = cache.values()
+    assert not ws.any()
+    ws[0] = 1
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert gdn_b200.binding.read_status() == 1 and gdn_b200.binding.read_status() == 0
+
+
 def test_streams_run_side_by_side():
     """Calls on two streams at once keep their own results."""
     g = gen(51)
