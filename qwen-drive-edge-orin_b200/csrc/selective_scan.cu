@@ -12,7 +12,9 @@
 namespace gdn {
 namespace ssm {
 
-// Up to this many tokens a prompt runs token by token. Measured (64 heads of 64, state 128, 64 sequences):
+// Calls of up to this many tokens a sequence run token by token, packed ones of up to this many token rows in all
+// (their lengths are on the device): 128 packed single tokens take the chunks, 408 us against 85 as a decode (64 heads
+// of 64). Measured (64 heads of 64, state 128, 64 sequences):
 // 115 us at 8 tokens and 197 at 16 against 194 for one chunk; one sequence of 24 heads: 6.0 and 10.3
 // against 9.8.
 constexpr int STEP_TOKENS = 15;

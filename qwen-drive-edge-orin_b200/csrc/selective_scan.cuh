@@ -1,5 +1,5 @@
 // Arguments of the selective scan, shared by its token-by-token kernel
-// (selective_scan_step.cu) and the chunked one (selective_scan.cu).
+// (selective_scan_step.cu) and the chunked one (selective_scan_chunk.cu).
 #pragma once
 
 #include <cuda_bf16.h>

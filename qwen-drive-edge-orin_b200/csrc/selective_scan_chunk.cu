@@ -25,7 +25,8 @@
 // what is of a chunk's size (output pass: the chunk's sum and the state's remainder beside its bf16 copy; state
 // pass: up to four chunks), which joins the rest in rounded fp32 additions. Final states of 65536 tokens of one
 // sign with almost no decay are off by 4e-6 of their value in one pass and 6e-6 in segments (7.6e-4 and 4.3e-5 with the whole
-// state as the accumulator; the steps that mend it cost 4%: 8 x 4096 x 64 heads 270 -> 283 us).
+// state as the accumulator; the steps that mend it cost 2 to 6%: 8 x 4096 x 64 heads 269 -> 275 us, 8 packed prompts
+// 158 -> 168).
 //
 // Decays are kept as base-2 logarithms, relative to 32-token blocks: e^{c_i - c_j} is a row factor times
 // a column factor, one exponential per row and block. Across blocks both are at most 1; inside a block
@@ -34,11 +35,13 @@
 // blocks, which take an exponential per element. (A third way was tried and left out: the row factors taken out of
 // M and applied to the finished row where a chunk decays by less than 2^64; no faster.)
 //
-// Measured on B200: 7.2 K cycles (4.2 us) per chunk and slot pair with one CTA on every SM, against 1.5 us for
-// the pair's 64 KB of x and y at the copy bandwidth; 8 x 4096 tokens of 64 heads of 64 in 264 us (256 CTAs in
-// two waves), token by token 6.3 ms. No unit is full (on the fullest SM: tensor pipe 50%, shared memory 48%;
-// issue slots 66% on its fullest quarter): two loops of dependent steps take the same time, G - M - scaling of y - M X - next G, and state
-// operand - output tile - X'^T - state product. What led here:
+// Measured on B200: 7.6 K cycles (4.4 us at 1.73 GHz) per chunk and slot pair with one CTA on every SM, against 1.5 us for
+// the pair's 64 KB of x and y at the copy bandwidth; 8 x 4096 tokens of 64 heads of 64 in 275 us at full clocks (256 CTAs in
+// two waves; 305 when the power cap holds the SMs at 1.76 GHz), token by token 6.3 ms. No unit is full (on the
+// fullest SM: tensor pipe 47%, shared memory 44%; issue slots 68% on its fullest quarter): two loops of dependent steps take about
+// the same time, G - M - scaling of y - M X - next G, and state operand - output tile - X'^T - state product. Slots are 64
+// channels wide, so P of 80 or 96 takes the time of 128, and P below 64 that of 64. What led here (times of the
+// version before the state's remainder):
 //   - shared memory feeds the MMAs' operands besides everything else (an MMA of 128 x 128 x 16 with both
 //     operands there takes all of its 128 bytes a cycle), so the two operands that the warps form, M and X'^T,
 //     are in TMEM;
@@ -194,7 +197,7 @@ __device__ __forceinline__ uint32_t row_at(uint32_t panel, int row) { return pan
 __device__ __forceinline__ void keep_local(uint32_t& v) { asm volatile("" : "+r"(v)); }
 // log(1 + e^v) = max(v, 0) + log(1 + e), e = e^-|v|, with log(1 + e) = 2 atanh(z), z = e / (2 + e) <= 1/3, by
 // its power series (the first term left out is below 2^-27 of the sum). Accurate relative to the result
-// for any v, in a third of the instructions of log1pf(expf(v)), whose eight copies a chunk the one gate
+// for v down to -87 (0 below, where e^v leaves fp32's normal range), in a third of the instructions of log1pf(expf(v)), whose eight copies a chunk the one gate
 // warp has no time for.
 __device__ __forceinline__ float softplus_series(float v) {
     float x = -fabsf(v);
@@ -1192,11 +1195,12 @@ ChunkPlan plan_scan_chunks(int N, int T, bool packed, int H, int P, int G, int s
     pl.segments = N;
     const int64_t rows = packed ? T : (int64_t)N * T;
     const int64_t chunks = N > 0 ? (rows / N + CH - 1) / CH : 0;  // of the mean sequence
-    // Wave model, measured on B200: an output pass takes 4.2 us per chunk and pair and 9.5 for a CTA's start
-    // and end, a state pass 1.8 and 5, the entry states 5. Segments pay where the (sequence, pair) units
-    // alone leave SMs idle (65536 tokens over 8 slots: 2.2 ms in one pass, 103 us in 37 segments). A
-    // packed batch's longest sequence is taken as twice the mean (the longest ones start first).
-    constexpr double OUT = 4.2, OUT_FIXED = 9.5, STATE = 1.8, STATE_FIXED = 5.0, ENTRY = 5.0;
+    // Wave model, measured on B200: an output pass takes 4.4 us per chunk and pair and 9.5 for a CTA's start
+    // and end, a state pass 2 and 5, the entry states 5. Segments pay where the (sequence, pair) units
+    // alone leave SMs idle (65536 tokens over 8 slots: 2.2 ms in one pass, 110 us in 37 segments). A
+    // packed batch's longest sequence is taken as twice the mean (the longest ones start first); a batch with one much
+    // longer prompt is not cut and takes that prompt's time (16384 beside 7 x 512, 64 heads of 64 in 8 groups: 510 us).
+    constexpr double OUT = 4.4, OUT_FIXED = 9.5, STATE = 2.0, STATE_FIXED = 5.0, ENTRY = 5.0;
     const int64_t ctas = (int64_t)N * pl.units;
     auto waves = [&](int64_t n) { return (double)((n + sms - 1) / sms); };
     const double one = OUT * chunks + OUT_FIXED;

@@ -55,8 +55,9 @@ __device__ __forceinline__ void stg(T* p, const Vec<T, VEC>& r) {
     }
 }
 
-// silu(v) = v / (1 + e^-v). 16-bit outputs take the fast exponential and division (a few fp32
-// ulp, far below the output's rounding); fp32 outputs the full-precision ones. e^-v = inf gives 0.
+// silu(v) = v / (1 + e^-v). 16-bit outputs take the fast exponential (off by 2 fp32 ulp and one more for each
+// unit of |v|: 2^-17 at most, far below the output's rounding) and division (0 for divisors above 2^126: below
+// v = -87.3, where silu is under 2^-119); fp32 outputs the full-precision ones. e^-v = inf gives 0.
 template <typename T>
 __device__ __forceinline__ float silu(float v) {
     if constexpr (sizeof(T) == 4) return v / (1.f + expf(-v));

@@ -285,8 +285,12 @@ def selective_scan_prefill(x, dt, A, B, C, D=None, dt_bias=None, s0=None, dt_sof
     x bf16 [B,T,H,P], dt fp32 or bf16 [B,T,H], B/C bf16 [B,T,G,N], A, D, dt_bias fp32 [H], initial
     state s0 fp32 [B,H,P,N] or zeros. P and N are multiples of 8 up to 128, B and H at most 65535, B T at
     most 2^31 - 129, and d A <= 0. A token with d = 0 (dt of minus infinity under the softplus) leaves the state as it is, so
-    padding in front of or between tokens is possible. An x that is not finite
+    padding in front of or between tokens (of finite x and B) is possible. An x that is not finite
     makes its channel's outputs NaN from the start of its 128 tokens (of its sequence) on.
+
+    Calls of 16 tokens and more run in chunks of 128 on the tensor cores: sums and the state are fp32, but two operands
+    of y, the weights of a chunk's tokens and the state at its start, are rounded to bf16 (as y is); the state is not
+    affected. Shorter calls are fp32 throughout.
     """
     return _scan_prefill(x, dt, A, B, C, D, dt_bias, s0, dt_softplus, None)
 
@@ -295,7 +299,8 @@ def selective_scan_prefill_varlen(x, dt, A, B, C, cu_seqlens, D=None, dt_bias=No
     """``selective_scan_prefill`` of packed sequences (B = 1): [y [1,T,H,P], final states [N,H,P,N]].
 
     ``cu_seqlens`` as in ``chunk_prefill_varlen``; sequence i starts from s0[i] or zeros. Tokens that
-    no sequence covers are not computed: their rows of y hold no defined values.
+    no sequence covers are not computed: their rows of y hold no defined values. Every sequence takes at least the
+    time of 128 tokens: the single tokens of many requests are faster through ``selective_scan_decode``.
     """
     return _scan_prefill(x, dt, A, B, C, D, dt_bias, s0, dt_softplus, cu_seqlens)
 
